@@ -151,6 +151,24 @@ DEVICE_ONLY_OP_SIGNATURES = {
 }
 STATIC_SCRATCH_BYTES = 8 << 20
 
+# operators of language models (no counterpart in the reference's interface either); `scratch, scratch_bytes` may be (None, 0)
+_SCRATCH = [C.c_void_p, C.c_size_t]
+MODEL_OP_SIGNATURES = {
+    "embedding": [_T, _T, _T, C.c_void_p],                                      # t, table, tokens, scale
+    "embedding_grad": [_T, _T, _T, C.c_void_p, C.c_int32] + _SCRATCH,           # d_table, tokens, d_out, scale, accumulate
+    "token_log_probs": [_T] * 7 + _SCRATCH,                                     # log_probs, lse, entropy, top_log_probs, top_tokens, logits, tokens
+    "token_log_probs_grad": [_T] * 7,                                           # d_logits, logits, tokens, lse, entropy, d_log_probs, d_entropy
+    "cross_attention": [_T] * 6 + [C.c_void_p] + _SCRATCH,                      # out, lse, q, k, v, mask, scale
+    "cross_attention_grad": [_T] * 10 + [C.c_void_p] + _SCRATCH,                # d_q, d_k, d_v, d_out, q, k, v, out, lse, mask, scale
+}
+# bytes of scratch memory they need; touch no device and take no stream
+_I64, _SZ = C.c_int64, P(C.c_size_t)
+SCRATCH_QUERY_SIGNATURES = {
+    "embedding_grad_scratch_bytes": [_I64, _I64, _I64, _SZ],                            # tokens, vocab, width
+    "token_log_probs_scratch_bytes": [C.c_int32, _I64, _I64, _I64, _SZ],                # dtype, rows, vocab, top
+    "cross_attention_scratch_bytes": [C.c_int32, _I64, _I64, _I64, _I64, _I64, _I64, _SZ],   # dtype, batch, heads, kv_heads, queries, keys, width
+}
+
 # every symbol include/tensor_hip.h declares
 EXPORTED_SYMBOLS = [
     "dnh_init", "dnh_device_info", "dnh_last_error", "dnh_async_error", "dnh_set_option", "dnh_get_option", "dnh_scatter_workspace_bytes",
@@ -159,4 +177,5 @@ EXPORTED_SYMBOLS = [
     "dnh_memcpy_h2d", "dnh_memcpy_d2h", "dnh_memcpy_d2d",
     "dnh_stream_create", "dnh_stream_destroy", "dnh_stream_sync", "dnh_device_sync",
     "dnh_event_create", "dnh_event_destroy", "dnh_event_record", "dnh_event_sync", "dnh_event_elapsed_ms",
-] + ["dnh_" + k for k in OP_SIGNATURES] + ["dnh_" + k for k in LAPACK_OP_SIGNATURES] + ["dnh_" + k for k in DEVICE_ONLY_OP_SIGNATURES]
+] + ["dnh_" + k for k in OP_SIGNATURES] + ["dnh_" + k for k in LAPACK_OP_SIGNATURES] + ["dnh_" + k for k in DEVICE_ONLY_OP_SIGNATURES] \
+  + ["dnh_" + k for k in MODEL_OP_SIGNATURES] + ["dnh_" + k for k in SCRATCH_QUERY_SIGNATURES]

@@ -24,6 +24,10 @@ std::mutex g_pinned_mu;
 std::map<uintptr_t, size_t> g_pinned;   // blocks handed out by dnh_host_alloc
 int g_cus = 256;
 std::map<hipStream_t, int32_t*> g_error_flags;   // one index-error word per stream, so concurrent streams do not see each other's errors
+// Words for g_error_flags, allocated and cleared once when the device is chosen: the first indexing call of a stream may be one that is
+// being captured into a graph, where nothing can be allocated.  A word goes back when its stream is destroyed.
+std::vector<int32_t*> g_spare_flags;
+constexpr int kSpareFlags = 1024;
 
 struct Workspace {
     std::mutex in_use;   // held through a WorkspaceLease while an entry point queues the kernels that use the buffer
@@ -107,6 +111,10 @@ static int32_t init_locked(int device) {
     hipDeviceProp_t prop;
     DNH_HIP(hipGetDeviceProperties(&prop, device));
     g_cus = prop.multiProcessorCount > 0 ? prop.multiProcessorCount : 256;
+    int32_t* flags = nullptr;
+    DNH_TRY(device_malloc((void**)&flags, kSpareFlags * sizeof(int32_t), "index error words"));
+    DNH_HIP(hipMemset(flags, 0, kSpareFlags * sizeof(int32_t)));   // synchronous: done before any kernel that may set one is queued
+    for (int i = kSpareFlags - 1; i >= 0; i--) g_spare_flags.push_back(flags + i);
     g_device = device;
     g_init = true;
     g_epoch.fetch_add(1, std::memory_order_release);
@@ -176,8 +184,13 @@ int32_t error_flag_ptr(hipStream_t stream, int32_t** out) {
     std::lock_guard<std::mutex> lock(g_mu);
     int32_t*& p = g_error_flags[stream];
     if (!p) {
-        DNH_TRY(device_malloc((void**)&p, sizeof(int32_t), "index error word"));
-        DNH_HIP(hipMemset(p, 0, sizeof(int32_t)));   // synchronous: done before any kernel that may set it is queued
+        if (!g_spare_flags.empty()) {
+            p = g_spare_flags.back();
+            g_spare_flags.pop_back();
+        } else {
+            DNH_TRY(device_malloc((void**)&p, sizeof(int32_t), "index error word"));
+            DNH_HIP(hipMemset(p, 0, sizeof(int32_t)));
+        }
     }
     *out = p;
     return DNH_OK;
@@ -257,7 +270,8 @@ static void drop_workspace(hipStream_t stream) {
     std::lock_guard<std::mutex> lock(g_mu);
     auto ef = g_error_flags.find(stream);
     if (ef != g_error_flags.end()) {
-        if (ef->second) (void)hipFree(ef->second);
+        // (the stream has been synchronised: nothing that could set the word is left)
+        if (ef->second && hipMemset(ef->second, 0, sizeof(int32_t)) == hipSuccess) g_spare_flags.push_back(ef->second);
         g_error_flags.erase(ef);
     }
     auto it = g_ws.find(stream);

@@ -13,7 +13,7 @@ import threading
 import numpy as np
 
 from . import abi, native
-from .backend import CAbiTensorBackend, ITensorDevice, ITensorStorage
+from .backend import CAbiTensorBackend, ITensorDevice, ITensorStorage, _scalar_buf
 from .layout import TensorLayout
 from . import layout as L
 from .tensor import Tensor
@@ -93,6 +93,56 @@ class TensorHipBackend(CAbiTensorBackend):
             code = C.c_int32(0)
             native.check(self._lib.dnh_async_error(Cfg.Stream, C.byref(code)))
             native.check(code.value)
+
+    # -- operators of language models (no counterpart in ITensorBackend; include/tensor_hip.h states their contracts) -----------------
+    # `scratch`: a contiguous tensor on the device for the call's intermediates, or None for the stream's workspace
+    @classmethod
+    def _opt(cls, t):
+        return None if t is None else C.byref(cls._desc(t))
+
+    @staticmethod
+    def _scale(value, dtype):
+        return (None, None) if value is None else _scalar_buf(value, dtype)
+
+    @staticmethod
+    def _scratch(t):
+        if t is None:
+            return None, 0
+        if not L.isC(t.Layout):
+            raise ValueError("scratch memory must be a contiguous tensor")
+        isz = t.Storage.DataType.itemsize
+        return t.Storage.Pointer() + t.Layout.Offset * isz, t.NElems * isz
+
+    def Embedding(self, trgt, table, tokens, scale=None):
+        keep, sp = self._scale(scale, table.Storage.DataType)
+        self._call("embedding", self._opt(trgt), self._opt(table), self._opt(tokens), sp)
+        self._after_indexed_op()
+
+    def EmbeddingGrad(self, trgt, tokens, dOut, scale=None, accumulate=False, scratch=None):
+        keep, sp = self._scale(scale, dOut.Storage.DataType)
+        self._call("embedding_grad", self._opt(trgt), self._opt(tokens), self._opt(dOut), sp, int(bool(accumulate)), *self._scratch(scratch))
+        self._after_indexed_op()
+
+    def TokenLogProbs(self, trgtLogProbs, trgtLse, trgtEntropy, trgtTopLogProbs, trgtTopTokens, logits, tokens, scratch=None):
+        self._call("token_log_probs", self._opt(trgtLogProbs), self._opt(trgtLse), self._opt(trgtEntropy), self._opt(trgtTopLogProbs),
+                   self._opt(trgtTopTokens), self._opt(logits), self._opt(tokens), *self._scratch(scratch))
+        if tokens is not None:
+            self._after_indexed_op()
+
+    def TokenLogProbsGrad(self, trgt, logits, tokens, lse, entropy, dLogProbs, dEntropy):
+        self._call("token_log_probs_grad", self._opt(trgt), self._opt(logits), self._opt(tokens), self._opt(lse), self._opt(entropy),
+                   self._opt(dLogProbs), self._opt(dEntropy))
+        self._after_indexed_op()
+
+    def CrossAttention(self, trgt, trgtLse, q, k, v, mask=None, scale=None, scratch=None):
+        keep, sp = self._scale(scale, q.Storage.DataType)
+        self._call("cross_attention", self._opt(trgt), self._opt(trgtLse), self._opt(q), self._opt(k), self._opt(v), self._opt(mask), sp,
+                   *self._scratch(scratch))
+
+    def CrossAttentionGrad(self, trgtQ, trgtK, trgtV, dOut, q, k, v, out, lse, mask=None, scale=None, scratch=None):
+        keep, sp = self._scale(scale, q.Storage.DataType)
+        self._call("cross_attention_grad", self._opt(trgtQ), self._opt(trgtK), self._opt(trgtV), self._opt(dOut), self._opt(q), self._opt(k),
+                   self._opt(v), self._opt(out), self._opt(lse), self._opt(mask), sp, *self._scratch(scratch))
 
     # single elements cross with a synchronous 1-element copy (CudaBackend.fs:77-93)
     def GetItem(self, idx):
@@ -215,6 +265,15 @@ def usingPtr(ptr: int, sizeInBytes: int, dtype, layout: TensorLayout) -> Tensor:
         if lo < 0 or hi >= nElems:
             raise ValueError(f"usingPtr: the layout addresses elements {lo}..{hi} but the allocation holds {nElems}")
     return Tensor(layout, TensorHipStorage(nElems, dt, Dev, external_ptr=int(ptr)))
+
+
+def scratchBytes(operator: str, *args) -> int:
+    """Bytes of scratch memory a call of a language-model operator needs (dnh_<operator>_scratch_bytes; an element type goes by its
+    NumPy type).  Touches no device."""
+    args = [abi.dtype_code(a) if isinstance(a, (type, np.dtype)) else int(a) for a in args]
+    n = C.c_size_t()
+    native.check(getattr(native.load(), f"dnh_{operator}_scratch_bytes")(*args, C.byref(n)))
+    return n.value
 
 
 def synchronize():

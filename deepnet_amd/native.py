@@ -61,8 +61,11 @@ def load() -> C.CDLL:
         "dnh_event_sync": [vp],
         "dnh_event_elapsed_ms": [vp, vp, C.POINTER(C.c_float)],
     }
-    for name, args in list(abi.OP_SIGNATURES.items()) + list(abi.LAPACK_OP_SIGNATURES.items()) + list(abi.DEVICE_ONLY_OP_SIGNATURES.items()):
-        sigs["dnh_" + name] = list(args) + [vp]  # every op takes the stream last
+    for ops in (abi.OP_SIGNATURES, abi.LAPACK_OP_SIGNATURES, abi.DEVICE_ONLY_OP_SIGNATURES, abi.MODEL_OP_SIGNATURES):
+        for name, args in ops.items():
+            sigs["dnh_" + name] = list(args) + [vp]  # every op takes the stream last
+    for name, args in abi.SCRATCH_QUERY_SIGNATURES.items():
+        sigs["dnh_" + name] = list(args)
     for name, args in sigs.items():
         fn = getattr(lib, name)
         fn.argtypes = args

@@ -727,6 +727,99 @@ class Tensor:
         trgt.FillDot(a, b)
         return trgt
 
+    # ---- operators of language models (no counterpart in Tensor.fs) ---------------------------------------------------------------------
+    # Forms as for every other operation: a static function that allocates its results, a Fill* form that writes into existing tensors.
+    # `scratch`: device memory for the intermediates of a call that is captured into a graph (hip.scratchBytes says how much).
+    def _model_op(self, name):
+        op = getattr(self.Backend, name, None)
+        if op is None:
+            raise NotImplementedError(f"{name} is not available on device {self.Dev.Id}")
+        return op
+
+    def FillEmbedding(self, table: "Tensor", tokens: "Tensor", scale=None):
+        """self[i, :] = scale * table[tokens[i], :]; scale defaults to 1."""
+        _same_storage([self, table, tokens])
+        self._model_op("Embedding")(self, table, tokens, scale)
+
+    @staticmethod
+    def embedding(table: "Tensor", tokens: "Tensor", scale=None) -> "Tensor":
+        if table.NDims != 2:
+            raise ValueError(f"An embedding table must be a matrix but it has shape {table.Shape}.")
+        trgt = Tensor.new(tokens.Shape + [table.Shape[1]], table.Dev, table.DataType)
+        trgt.FillEmbedding(table, tokens, scale)
+        return trgt
+
+    def FillEmbeddingGrad(self, tokens: "Tensor", dOut: "Tensor", scale=None, accumulate=False, scratch=None):
+        """self[v, :] = scale * sum of dOut[i, :] over the i with tokens[i] = v; accumulate=True adds that to self."""
+        _same_storage([self, tokens, dOut])
+        self._model_op("EmbeddingGrad")(self, tokens, dOut, scale, accumulate, scratch)
+
+    @staticmethod
+    def embeddingGrad(tokens: "Tensor", dOut: "Tensor", vocab: int, scale=None) -> "Tensor":
+        if dOut.NDims < 1:
+            raise ValueError("dOut needs a last axis of the table's row length.")
+        trgt = Tensor.new([vocab, dOut.Shape[-1]], dOut.Dev, dOut.DataType)
+        trgt.FillEmbeddingGrad(tokens, dOut, scale)
+        return trgt
+
+    @staticmethod
+    def FillTokenLogProbs(logits: "Tensor", tokens=None, logProbs=None, lse=None, entropy=None, topLogProbs=None, topTokens=None, scratch=None):
+        """Fills the given targets from logits [i_1 .. i_n; V]: log probabilities of tokens [i], lse and entropy [i] of each row, the
+        largest log probabilities and their tokens [i; K]."""
+        _same_storage([logits, tokens, logProbs, lse, entropy, topLogProbs, topTokens])
+        logits._model_op("TokenLogProbs")(logProbs, lse, entropy, topLogProbs, topTokens, logits, tokens, scratch)
+
+    @staticmethod
+    def tokenLogProbs(logits: "Tensor", tokens: "Tensor", top: int = 0):
+        """(logProbs, lse, entropy), followed by (topLogProbs, topTokens) when top > 0."""
+        new = lambda shp, dt: Tensor.new(shp, logits.Dev, dt)
+        row = logits.Shape[:-1]
+        out = [new(row, logits.DataType) for _ in range(3)]
+        if top:
+            out += [new(row + [top], logits.DataType), new(row + [top], np.int64)]
+        Tensor.FillTokenLogProbs(logits, tokens, *out)
+        return tuple(out)
+
+    def FillTokenLogProbsGrad(self, logits, tokens, lse, dLogProbs, entropy=None, dEntropy=None):
+        """self = gradient of sum(dLogProbs logProbs + dEntropy entropy) with respect to logits; self may be logits."""
+        _same_storage([self, logits, tokens, lse, dLogProbs, entropy, dEntropy])
+        self._model_op("TokenLogProbsGrad")(self, logits, tokens, lse, entropy, dLogProbs, dEntropy)
+
+    @staticmethod
+    def tokenLogProbsGrad(logits, tokens, lse, dLogProbs, entropy=None, dEntropy=None) -> "Tensor":
+        trgt = Tensor.new(logits.Shape, logits.Dev, logits.DataType)
+        trgt.FillTokenLogProbsGrad(logits, tokens, lse, dLogProbs, entropy, dEntropy)
+        return trgt
+
+    def FillCrossAttention(self, q, k, v, mask=None, scale=None, lse=None, scratch=None):
+        """self = softmax(scale q k^T) v over the keys for which mask [batch; position] is true, lse the logarithm of each row's sum of
+        exponentials.  q [batch; head; position; width]; k and v may have fewer heads, each shared by neighbouring query heads."""
+        _same_storage([self, q, k, v, mask, lse])
+        self._model_op("CrossAttention")(self, lse, q, k, v, mask, scale, scratch)
+
+    @staticmethod
+    def crossAttention(q, k, v, mask=None, scale=None):
+        """(out, lse)"""
+        if q.NDims != 4 or v.NDims != 4:
+            raise ValueError(f"q and v must have the axes [batch; head; position; width], but have shapes {q.Shape} and {v.Shape}.")
+        out = Tensor.new(q.Shape[:3] + [v.Shape[3]], q.Dev, q.DataType)
+        lse = Tensor.new(q.Shape[:3], q.Dev, q.DataType)
+        out.FillCrossAttention(q, k, v, mask, scale, lse)
+        return out, lse
+
+    @staticmethod
+    def FillCrossAttentionGrad(dQ, dK, dV, dOut, q, k, v, out, lse, mask=None, scale=None, scratch=None):
+        """Gradients of sum(dOut out) into dQ, dK and dV; dQ, or dK and dV, may be None."""
+        _same_storage([dQ, dK, dV, dOut, q, k, v, out, lse, mask])
+        q._model_op("CrossAttentionGrad")(dQ, dK, dV, dOut, q, k, v, out, lse, mask, scale, scratch)
+
+    @staticmethod
+    def crossAttentionGrad(dOut, q, k, v, out, lse, mask=None, scale=None):
+        """(dQ, dK, dV)"""
+        dQ, dK, dV = (Tensor.new(t.Shape, t.Dev, t.DataType) for t in (q, k, v))
+        Tensor.FillCrossAttentionGrad(dQ, dK, dV, dOut, q, k, v, out, lse, mask, scale)
+        return dQ, dK, dV
+
     # ---- comparison helpers (Tensor.fs:3901-3925) -----------------------------------------------------------------------------------------------------------
     def isClose(self, b: "Tensor", absTol=1e-8, relTol=1e-5) -> "Tensor":
         """|a-b| <= absTol + relTol*|b| for float types, exact equality otherwise."""

@@ -328,6 +328,64 @@ int32_t dnh_batched_svd(const DnhTensor* s, const DnhTensor* u, const DnhTensor*
  * column k of eigvecs [n; n] the unit eigenvector of eigenvalue k.  eigvecs may be src. */
 int32_t dnh_symmetric_eig(int32_t part, const DnhTensor* eigvals, const DnhTensor* eigvecs, const DnhTensor* src, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------
+ * Operators of language models (no counterpart in ITensorBackend): token embedding, token log probabilities, cross attention, each
+ * with its gradient.  Single and double precision, int64 tokens, any strides and offsets.
+ *  - `scale` points to one host element of the operands' type, as `value` of dnh_fill_const does; NULL selects the default;
+ *  - targets may not be broadcast views and, unless a declaration says so, may not overlap a source;
+ *  - `scratch` is device memory for the call's intermediates, aligned to 16 bytes, of at least the number of bytes that the
+ *    operator's dnh_*_scratch_bytes reports; it must stay untouched until the call's kernels have run.  NULL: the library uses the
+ *    stream's workspace.  While the stream is being captured into a graph, a call that needs scratch memory is refused without it
+ *    (DNH_ERR_INVALID_ARG): a graph keeps the addresses it was captured with, whereas the workspace moves when it grows and belongs
+ *    to everything on the stream.  Two graphs that may run at the same time need scratch memory of their own each;
+ *  - no result depends on the order of atomics: the same call gives the same bits every time.
+ * ------------------------------------------------------------------------------------------------- */
+/* t[i, :] = scale * table[tokens[i], :].  table [V; D], tokens [i_1 .. i_n], t [i_1 .. i_n; D]; scale defaults to 1.  One product,
+ * rounded once.  A token outside the table sets the stream's error flag (dnh_async_error) and leaves its row of t unwritten. */
+int32_t dnh_embedding(const DnhTensor* t, const DnhTensor* table, const DnhTensor* tokens_i64, const void* scale, void* stream);
+/* d_table[v, :] = scale * sum of d_out[i, :] over the i with tokens[i] = v, for every row v (accumulate = 0: rows of absent tokens
+ * become zero), or that sum added to d_table (accumulate = 1: rows of absent tokens stay untouched).  The tokens are sorted and each
+ * row's addends summed in double precision, in an order that depends on the tokens alone; one rounding at the end.  A token outside
+ * the table sets the stream's error flag and contributes nothing.  Up to 2^27 tokens. */
+int32_t dnh_embedding_grad(const DnhTensor* d_table, const DnhTensor* tokens_i64, const DnhTensor* d_out, const void* scale, int32_t accumulate,
+                           void* scratch, size_t scratch_bytes, void* stream);
+int32_t dnh_embedding_grad_scratch_bytes(int64_t tokens, int64_t vocab, int64_t width, size_t* bytes);
+/* From logits [i_1 .. i_n; V], per row and in one pass over them:
+ *   lse [i]              log of the sum of e^logit
+ *   log_probs [i]        logits[i, tokens[i]] - lse; given together with tokens
+ *   entropy [i]          -sum p log p of p = e^(logit - lse)
+ *   top_log_probs, top_tokens [i; K]   the K largest logits as log probabilities and their int64 indices in descending order,
+ *                        equal ones by ascending index, K <= 64 and <= V; given together
+ * Any of the targets may be NULL, at least one is needed.  A logit of -inf has probability 0 and adds nothing to the entropy.  A row
+ * whose logits are all -inf has lse, log_probs and top_log_probs -inf and entropy 0.  NaN or +inf in a row gives NaN in its lse,
+ * log_probs, entropy and top_log_probs; a NaN is no alternative (top_tokens is DNH_NOT_FOUND where fewer than K numbers are left).
+ * A token outside 0 .. V - 1 sets the stream's error flag and leaves its log_probs element unwritten. */
+int32_t dnh_token_log_probs(const DnhTensor* log_probs, const DnhTensor* lse, const DnhTensor* entropy, const DnhTensor* top_log_probs,
+                            const DnhTensor* top_tokens_i64, const DnhTensor* logits, const DnhTensor* tokens_i64, void* scratch, size_t scratch_bytes,
+                            void* stream);
+int32_t dnh_token_log_probs_scratch_bytes(int32_t dtype, int64_t rows, int64_t vocab, int64_t top, size_t* bytes);
+/* d_logits[i, j] = g[i] (1[j = tokens[i]] - p_j) - h[i] p_j (log p_j + entropy[i]) with p_j = e^(logits[i, j] - lse[i]), g = d_log_probs
+ * and h = d_entropy: the gradient of sum(g log_probs + h entropy).  entropy and d_entropy are given together or are both NULL.
+ * d_logits may be logits (same layout): it is then overwritten in place.  Rows whose lse is -inf get zeros.  A token outside
+ * 0 .. V - 1 sets the stream's error flag and leaves its row of d_logits unwritten. */
+int32_t dnh_token_log_probs_grad(const DnhTensor* d_logits, const DnhTensor* logits, const DnhTensor* tokens_i64, const DnhTensor* lse,
+                                 const DnhTensor* entropy, const DnhTensor* d_log_probs, const DnhTensor* d_entropy, void* stream);
+/* out = softmax(scale q k^T) v over the keys that the mask leaves, lse = log of the sum of e^(scale q.k).
+ * q [B; Hq; Lq; Dk], k [B; Hk; Lk; Dk], v [B; Hk; Lk; Dv], out [B; Hq; Lq; Dv], lse [B; Hq; Lq] or NULL.  Hq is a multiple of Hk: query
+ * head h reads key head h / (Hq / Hk).  mask [B; Lk] (bool) or NULL: keys with false are not attended to, and what k and v hold there
+ * (infinities and NaN included) is not read.  A sequence without keys has out 0 and lse -inf.  scale defaults to 1 / sqrt(Dk).
+ * Widths up to 128.  [B; L; H; D] tensors are passed as permuted views. */
+int32_t dnh_cross_attention(const DnhTensor* out, const DnhTensor* lse, const DnhTensor* q, const DnhTensor* k, const DnhTensor* v,
+                            const DnhTensor* mask_bool, const void* scale, void* scratch, size_t scratch_bytes, void* stream);
+/* Gradients of sum(d_out out) with out and lse as dnh_cross_attention gave them: d_q like q, d_k like k, d_v like v, those of a shared key
+ * head summed over its query heads, those of masked keys zero.  d_q, or d_k and d_v, may be NULL. */
+int32_t dnh_cross_attention_grad(const DnhTensor* d_q, const DnhTensor* d_k, const DnhTensor* d_v, const DnhTensor* d_out, const DnhTensor* q,
+                                 const DnhTensor* k, const DnhTensor* v, const DnhTensor* out, const DnhTensor* lse, const DnhTensor* mask_bool,
+                                 const void* scale, void* scratch, size_t scratch_bytes, void* stream);
+/* Scratch memory that either direction needs (width: that of v). */
+int32_t dnh_cross_attention_scratch_bytes(int32_t dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t queries, int64_t keys, int64_t width,
+                                          size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif
