@@ -84,7 +84,7 @@ AttArgs<T> common_args(const DnhTensor* q, const DnhTensor* k, const DnhTensor* 
     p.Dv = (int)v->shape[3];
     p.rows = (uint32_t)p.G * (uint32_t)p.Lq;
     p.scale = scalar_arg<T>(scale, 1.0 / sqrt((double)p.Dk));
-    p.scale_base = (T)((double)p.scale * Mma<T>::kBase);
+    p.scale_base = (T)((double)p.scale * MmaOf<T>::Tile::kBase);
     p.vec = p.sq.d == 1 && p.sk.d == 1 && p.sv.d == 1;
     return p;
 }
@@ -136,7 +136,7 @@ extern "C" int32_t dnh_cross_attention_scratch_bytes(int32_t dtype, int64_t batc
     *bytes = 0;
     if (n == 0 || rows == 0) return DNH_OK;
     const size_t f = dtype == DNH_F32 ? att_plan<float>(n, rows, keys, width).total : att_plan<double>(n, rows, keys, width).total;
-    const size_t b = up256((size_t)n * rows * dtype_size(dtype));
+    const size_t b = dtype == DNH_F32 ? att_grad_plan<float>(n, rows, keys, width, width).total : att_grad_plan<double>(n, rows, keys, width, width).total;
     *bytes = f > b ? f : b;
     return DNH_OK;
 }

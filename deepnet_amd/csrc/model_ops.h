@@ -4,6 +4,8 @@
 
 #include "common.h"
 
+#include <type_traits>
+
 namespace dnh {
 
 // 16 bytes of T at T's own alignment (the hardware serves 16-byte accesses at any dword address, so views that start at an odd

@@ -373,7 +373,7 @@ int32_t dnh_token_log_probs_grad(const DnhTensor* d_logits, const DnhTensor* log
 /* out = softmax(scale q k^T) v over the keys that the mask leaves, lse = log of the sum of e^(scale q.k).
  * q [B; Hq; Lq; Dk], k [B; Hk; Lk; Dk], v [B; Hk; Lk; Dv], out [B; Hq; Lq; Dv], lse [B; Hq; Lq] or NULL.  Hq is a multiple of Hk: query
  * head h reads key head h / (Hq / Hk).  mask [B; Lk] (bool) or NULL: keys with false are not attended to, and what k and v hold there
- * (infinities and NaN included) is not read.  A sequence without keys has out 0 and lse -inf.  scale defaults to 1 / sqrt(Dk).
+ * (infinities and NaN included) is not used.  A sequence without keys has out 0 and lse -inf.  scale defaults to 1 / sqrt(Dk).
  * Widths up to 128.  [B; L; H; D] tensors are passed as permuted views. */
 int32_t dnh_cross_attention(const DnhTensor* out, const DnhTensor* lse, const DnhTensor* q, const DnhTensor* k, const DnhTensor* v,
                             const DnhTensor* mask_bool, const void* scale, void* scratch, size_t scratch_bytes, void* stream);
@@ -382,7 +382,7 @@ int32_t dnh_cross_attention(const DnhTensor* out, const DnhTensor* lse, const Dn
 int32_t dnh_cross_attention_grad(const DnhTensor* d_q, const DnhTensor* d_k, const DnhTensor* d_v, const DnhTensor* d_out, const DnhTensor* q,
                                  const DnhTensor* k, const DnhTensor* v, const DnhTensor* out, const DnhTensor* lse, const DnhTensor* mask_bool,
                                  const void* scale, void* scratch, size_t scratch_bytes, void* stream);
-/* Scratch memory that either direction needs (width: that of v). */
+/* Scratch memory that either direction needs; width: the larger one of Dk and Dv. */
 int32_t dnh_cross_attention_scratch_bytes(int32_t dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t queries, int64_t keys, int64_t width,
                                           size_t* bytes);
 
