@@ -86,6 +86,13 @@ AttArgs<T> common_args(const DnhTensor* q, const DnhTensor* k, const DnhTensor* 
     p.scale = scalar_arg<T>(scale, 1.0 / sqrt((double)p.Dk));
     p.scale_base = (T)((double)p.scale * MmaOf<T>::Tile::kBase);
     p.vec = p.sq.d == 1 && p.sk.d == 1 && p.sv.d == 1;
+    p.whole = p.vec && p.Dk % kVecN<T> == 0 && p.Dv % kVecN<T> == 0;
+    // with 2^(l - 1) < Lq <= 2^l and mul = ceil(2^(31 + l) / Lq): mul Lq exceeds 2^(31 + l) by less than 2^l, so r mul 2^-(31 + l) exceeds
+    // r / Lq by less than r 2^-31 / Lq < 1 / Lq, and the integer parts agree
+    int l = 0;
+    while (((int64_t)1 << l) < p.Lq) l++;
+    p.lq_shift = 31 + l;
+    p.lq_mul = p.Lq > 0 ? (uint32_t)((((uint64_t)1 << (31 + l)) + p.Lq - 1) / p.Lq) : 0;
     return p;
 }
 
@@ -113,6 +120,7 @@ int32_t backward(const DnhTensor* dq, const DnhTensor* dk, const DnhTensor* dv, 
     p.lse = (const T*)elem_ptr(lse);
     p.slse = strides4(lse);
     p.vec = p.vec && p.sdo.d == 1;
+    p.whole = p.whole && p.vec;
     if (dq) {
         p.dq = (T*)elem_ptr(dq);
         p.sdq = strides4(dq);

@@ -75,8 +75,11 @@ template <class T> struct AttArgs {
     int64_t mask_b, mask_l;
     int B, Hk, G, Lq, Lk, Dk, Dv;
     uint32_t rows;            // G Lq
+    uint32_t lq_mul;          // r / Lq = r lq_mul >> lq_shift for r < 2^31
+    int lq_shift;
     T scale, scale_base;      // scale, and scale x log e in the exponentials' base
     bool vec;                 // q, k, v (and d_out) are contiguous along their last axis
+    bool whole;               // and their widths are whole 16-byte pieces
     // workgroups of a key head: row blocks x shares of the keys (forward, dq), key blocks x shares of the rows (dk, dv)
     uint32_t blocks, splits, split_tiles;
     uint32_t kblocks, ksplits, ksplit_tiles;
@@ -114,6 +117,18 @@ __device__ __forceinline__ typename Vec16<T>::type att_load(const T* row, int d,
     return v;
 }
 
+// The same without a branch (which would make every load wait for the one before it), for rows that are contiguous and hold whole pieces
+template <class T, bool WHOLE>
+__device__ __forceinline__ typename Vec16<T>::type att_piece(const T* row, int d, int D, int64_t sd, bool vec) {
+    using V = typename Vec16<T>::type;
+    if constexpr (WHOLE) {
+        const V v = *(const V*)(row + (d < D ? d : 0));
+        return d < D ? v : V(0);
+    } else {
+        return att_load<T>(row, d, D, sd, vec);
+    }
+}
+
 template <class T, int DP> constexpr int kAttPitch = DP + kVecN<T>;   // LDS rows: 16 rows' 16-byte reads fall on different banks
 
 template <class T> __device__ __forceinline__ bool att_key_on(const AttArgs<T>& p, int b, int key) {
@@ -131,37 +146,40 @@ __device__ __forceinline__ void att_words(const AttArgs<T>& p, int b, int t0, in
     }
 }
 
-// A tile of 32 rows of two matrices on its way from memory to LDS: loaded into registers while the tile before it is worked on.
-template <class T, int DP, int WAVES> struct AttStage {
+// A tile of 32 rows of two matrices on its way from memory to LDS: loaded into registers while the tile before it is worked on.  WHOLE:
+// rows are contiguous and hold whole 16-byte pieces; the loads are then straight-line code whose results nothing touches before
+// store() (a branch between two ways of loading would make the compiler wait for the data where the ways meet).
+template <class T, int DP, int WAVES, bool WHOLE> struct AttStage {
     using V = typename Vec16<T>::type;
     static constexpr int N = kVecN<T>, PER = DP / N, NL = kAttTile * PER / (64 * WAVES);
     static_assert(NL * 64 * WAVES == kAttTile * PER, "the workgroup covers a tile evenly");
     V a[NL], b[NL];
-    // row(r, which): address of row r of the tile (always readable); rows whose bit is not set become zeros
-    template <class Row>
-    __device__ __forceinline__ void load(Row row, int Da, int Db, int64_t sda, int64_t sdb, bool vec, uint32_t word) {
-        const bool whole = vec && Da == DP && Db == DP;
+    // row(r, which): address of row r of the tile (always readable)
+    template <class Row> __device__ __forceinline__ void load(Row row, int Da, int Db, int64_t sda, int64_t sdb, bool vec) {
 #pragma unroll
         for (int j = 0; j < NL; j++) {
             const int i = threadIdx.x + j * 64 * WAVES, r = i / PER, d = (i - r * PER) * N;
             const T *pa = row(r, 0), *pb = row(r, 1);
-            if (whole) {
-                a[j] = *(const V*)(pa + d);
-                b[j] = *(const V*)(pb + d);
+            if constexpr (WHOLE) {
+                a[j] = *(const V*)(pa + (d < Da ? d : 0));
+                b[j] = *(const V*)(pb + (d < Db ? d : 0));
             } else {
                 a[j] = att_load<T>(pa, d, Da, sda, vec);
                 b[j] = att_load<T>(pb, d, Db, sdb, vec);
             }
         }
-        if (word != ~0u) {
+    }
+    // rows whose bit is not set, and what lies beyond the width, become zeros
+    __device__ __forceinline__ void store(T* la, T* lb, int Da, int Db, uint32_t word) {
+        if (word != ~0u || Da < DP || Db < DP) {
 #pragma unroll
             for (int j = 0; j < NL; j++) {
-                const int r = (threadIdx.x + j * 64 * WAVES) / PER;
-                if (!((word >> r) & 1u)) a[j] = b[j] = 0;
+                const int i = threadIdx.x + j * 64 * WAVES, r = i / PER, d = (i - r * PER) * N;
+                const bool on = (word >> r) & 1u;
+                if (!on || d >= Da) a[j] = 0;
+                if (!on || d >= Db) b[j] = 0;
             }
         }
-    }
-    __device__ __forceinline__ void store(T* la, T* lb) const {
 #pragma unroll
         for (int j = 0; j < NL; j++) {
             const int i = threadIdx.x + j * 64 * WAVES, r = i / PER, d = (i - r * PER) * N;
@@ -190,11 +208,138 @@ template <class T>
 __device__ __forceinline__ int64_t att_row(const AttArgs<T>& p, const Strides4& s, int b, int hk, uint32_t r) {
     uint32_t g = 0, i = r;
     if (p.G > 1) {
-        g = r / (uint32_t)p.Lq;
+        g = (uint32_t)(((uint64_t)r * p.lq_mul) >> p.lq_shift);   // r / Lq
         i = r - g * (uint32_t)p.Lq;
     }
     return b * s.b + (int64_t)(hk * p.G + (int)g) * s.h + (int64_t)i * s.l;
 }
+
+// ---- products of one staged tile ------------------------------------------------------------------------------------------------------
+// The compiler, left alone, reads an operand from LDS right before the instructions that use it and waits; with one or two wavefronts on
+// a SIMD the matrix pipe then idles for the LDS latency each time.  Here every read is issued one or two groups of instructions
+// ahead, and scheduling barriers (which let ordinary vector and scalar instructions pass) keep it there.
+//
+// Result accumulators: lane row i of accumulator n holds element d_of(n, i) of the width, chosen so that a lane's operands for E
+// accumulators are neighbours in LDS (one read) and its results are neighbours in memory.
+template <class A, int DP> struct AttOps {
+    using Mma = A;
+    using T = typename A::T;
+    using V = typename Vec16<T>::type;
+    using Acc = typename A::Acc;
+    static constexpr int M = A::M, N = A::N, GN = A::G * N, NT = DP / GN, NS = kAttTile / M, ND = DP / M, P = kAttPitch<T, DP>;
+    static constexpr int E = ND % N == 0 ? N : ND == 2 ? 2 : 1, NE = ND / E;
+    typedef T VE __attribute__((ext_vector_type(E)));
+    static __device__ __forceinline__ int d_of(int n, int i) { return (n / E) * (M * E) + E * i + n % E; }
+    static __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0x6); }
+
+    // a lane's column of the result, times f, to a row of D elements
+    static __device__ __forceinline__ void put(T* row, int64_t sd, int D, const Acc (&o)[ND], T f, int h) {
+        if (E > 1 && sd == 1 && D % E == 0) {
+            typedef T VU __attribute__((ext_vector_type(E), aligned(sizeof(T))));   // E neighbours at the element's alignment
+#pragma unroll
+            for (int n = 0; n < ND; n += E)
+#pragma unroll
+                for (int r = 0; r < A::R; r++) {
+                    const int d = d_of(n, A::acc_row(r, h));
+                    VU v;
+#pragma unroll
+                    for (int e = 0; e < E; e++) v[e] = o[n + e][r] * f;
+                    if (d < D) *(VU*)(row + d) = v;
+                }
+            return;
+        }
+#pragma unroll
+        for (int n = 0; n < ND; n++)
+#pragma unroll
+            for (int r = 0; r < A::R; r++) {
+                const int d = d_of(n, A::acc_row(r, h));
+                if (d < D) row[d * sd] = o[n][r] * f;
+            }
+    }
+    // s = rows of the tile . x; at: the tile's element [c][h N]
+    static __device__ __forceinline__ void scores(Acc& s, const T* at, const V (&x)[NT]) {
+        V a[2];
+        a[0] = *(const V*)at;
+        s = 0;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (t + 1 < NT) a[(t + 1) & 1] = *(const V*)(at + GN * (t + 1));
+            pin();
+#pragma unroll
+            for (int e = 0; e < N; e++) s = A::mfma(a[t & 1][e], x[t][e], s);
+            pin();
+        }
+    }
+    // two at once
+    static __device__ __forceinline__ void scores(Acc& s, const T* at, const V (&x)[NT], Acc& z, const T* zat, const V (&y)[NT]) {
+        V a[2], w[2];
+        a[0] = *(const V*)at;
+        w[0] = *(const V*)zat;
+        s = 0;
+        z = 0;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (t + 1 < NT) {
+                a[(t + 1) & 1] = *(const V*)(at + GN * (t + 1));
+                w[(t + 1) & 1] = *(const V*)(zat + GN * (t + 1));
+            }
+            pin();
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                s = A::mfma(a[t & 1][e], x[t][e], s);
+                z = A::mfma(w[t & 1][e], y[t][e], z);
+            }
+            pin();
+        }
+    }
+    // operands of step x (of NS R): the tile's row that register x % R of sub-tile x / R stands for; at: element [0][E c]
+    struct Row {
+        VE v[NE];
+        __device__ __forceinline__ void read(const T* at, int x, int h) {
+            const T* r = at + ((x / A::R) * M + A::acc_row(x % A::R, h)) * P;
+#pragma unroll
+            for (int n = 0; n < NE; n++) v[n] = *(const VE*)(r + n * M * E);
+        }
+        __device__ __forceinline__ T operator[](int n) const {
+            if constexpr (E == 1) return v[n][0];
+            else return v[n / E][n % E];
+        }
+    };
+    // o += (rows of the tile)^T . s for steps [x0, x0 + R) of the tile, s: the sub-tile's registers; first: Row 0 and 1 of those steps
+    static __device__ __forceinline__ void outer(Acc (&o)[ND], const T* at, int x0, int h, const Acc& s) {
+        Row a[3];
+        a[0].read(at, x0, h);
+        a[1].read(at, x0 + 1, h);
+#pragma unroll
+        for (int r = 0; r < A::R; r++) {
+            if (r + 2 < A::R) a[(r + 2) % 3].read(at, x0 + r + 2, h);
+            pin();
+#pragma unroll
+            for (int n = 0; n < ND; n++) o[n] = A::mfma(a[r % 3][n], s[r], o[n]);
+            pin();
+        }
+    }
+    // two at once
+    static __device__ __forceinline__ void outer(Acc (&o)[ND], const T* at, const Acc& s, Acc (&z)[ND], const T* zat, const Acc& y, int x0, int h) {
+        Row a[2], w[2];
+        a[0].read(at, x0, h);
+        w[0].read(zat, x0, h);
+#pragma unroll
+        for (int r = 0; r < A::R; r++) {
+            if (r + 1 < A::R) {
+                a[(r + 1) & 1].read(at, x0 + r + 1, h);
+                w[(r + 1) & 1].read(zat, x0 + r + 1, h);
+            }
+            pin();
+#pragma unroll
+            for (int n = 0; n < ND; n++) {
+                o[n] = A::mfma(a[r & 1][n], s[r], o[n]);
+                z[n] = A::mfma(w[r & 1][n], y[r], z[n]);
+            }
+            pin();
+        }
+    }
+};
 
 // ---- the softmax of one tile ----------------------------------------------------------------------------------------------------------
 // s: scores S^T of NS sub-tiles, becomes probabilities relative to the running maximum m; l is this lane's share of the sum.  Returns the
@@ -238,29 +383,18 @@ template <class A> __device__ __forceinline__ typename A::T att_lse_of(typename 
     return l == T(0) ? -(T)__builtin_inf() : (T)((m + A::log_(l)) * (T)(1.0 / A::kBase));
 }
 
-// Stores a wavefront's result out^T (lane: row, registers: width) or its share of it; d_of(i, r) is the element that register r of
-// accumulator i holds.
-template <class A, int ND, class DOf>
-__device__ __forceinline__ void att_store(const AttArgs<typename A::T>& p, const typename A::Acc (&o)[ND], DOf d_of, uint32_t head, int b, int hk, uint32_t row,
-                                          uint32_t split, int h, typename A::T m, typename A::T l) {
-    using T = typename A::T;
+// Stores a wavefront's result out^T (lane: row, registers: width) or its share of it.
+template <class Ops>
+__device__ __forceinline__ void att_store(const AttArgs<typename Ops::T>& p, const typename Ops::Acc (&o)[Ops::ND], uint32_t head, int b, int hk, uint32_t row,
+                                          uint32_t split, int h, typename Ops::T m, typename Ops::T l) {
+    using T = typename Ops::T;
     if (p.splits == 1) {
-        const T inv = l == T(0) ? T(0) : T(1) / l;   // a row that attends to nothing is zero
-        T* orow = p.o + att_row(p, p.so, b, hk, row);
-#pragma unroll
-        for (int i = 0; i < ND; i++)
-#pragma unroll
-            for (int r = 0; r < A::R; r++)
-                if (d_of(i, r) < p.Dv) orow[d_of(i, r) * p.so.d] = o[i][r] * inv;
-        if (p.lse_out && h == 0) p.lse_out[att_row(p, p.slse, b, hk, row)] = att_lse_of<A>(m, l);
+        Ops::put(p.o + att_row(p, p.so, b, hk, row), p.so.d, p.Dv, o, l == T(0) ? T(0) : T(1) / l, h);   // a row that attends to nothing is zero
+        if (p.lse_out && h == 0) p.lse_out[att_row(p, p.slse, b, hk, row)] = att_lse_of<typename Ops::Mma>(m, l);
         return;
     }
     const size_t at = ((size_t)head * p.rows + row) * p.splits + split;
-#pragma unroll
-    for (int i = 0; i < ND; i++)
-#pragma unroll
-        for (int r = 0; r < A::R; r++)
-            if (d_of(i, r) < p.Dv) p.part_o[at * p.Dv + d_of(i, r)] = o[i][r];
+    Ops::put(p.part_o + at * p.Dv, 1, p.Dv, o, T(1), h);
     if (h == 0) {
         p.part_m[at] = m;
         p.part_l[at] = l;
@@ -271,12 +405,13 @@ __device__ __forceinline__ void att_store(const AttArgs<typename A::T>& p, const
 // A wavefront owns M rows and keeps their queries in registers; the workgroup's wavefronts share the keys and values, which go through
 // two LDS buffers: the next tile's loads are in flight while this one is worked on, and one barrier per tile suffices (a wavefront
 // that writes buffer b has passed the barrier behind everybody's last reads of it).
-template <class A, int DP, int WAVES>
+template <class A, int DP, int WAVES, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel(AttArgs<typename A::T> p) {
     using T = typename A::T;
     using V = typename Vec16<T>::type;
     using Acc = typename A::Acc;
     constexpr int M = A::M, N = A::N, GN = A::G * N, NT = DP / GN, NS = kAttTile / M, ND = DP / M, P = kAttPitch<T, DP>;
+    using Ops = AttOps<A, DP>;
     __shared__ __attribute__((aligned(16))) T Ks[2][kAttTile * P];
     __shared__ __attribute__((aligned(16))) T Vs[2][kAttTile * P];
     __shared__ uint32_t words[kAttWords];
@@ -290,7 +425,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel
     const T* qr = p.q + att_row(p, p.sq, b, hk, live ? row : 0);
     V q[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) q[t] = att_load<T>(qr, GN * t + h * N, p.Dk, p.sq.d, p.vec);
+    for (int t = 0; t < NT; t++) q[t] = att_piece<T, WHOLE>(qr, GN * t + h * N, p.Dk, p.sq.d, p.vec);
     Acc o[ND];
 #pragma unroll
     for (int i = 0; i < ND; i++) o[i] = 0;
@@ -299,7 +434,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel
     const int t0 = split * p.split_tiles, t1 = tiles < (int)(t0 + p.split_tiles) ? tiles : (int)(t0 + p.split_tiles);
     const T* kb = p.k + b * p.sk.b + hk * p.sk.h;
     const T* vb = p.v + b * p.sv.b + hk * p.sv.h;
-    AttStage<T, DP, WAVES> st;
+    AttStage<T, DP, WAVES, WHOLE> st;
     for (int w0 = t0; w0 < t1; w0 += kAttWords) {
         const int wn = t1 - w0 < kAttWords ? t1 - w0 : kAttWords;
         __syncthreads();
@@ -314,58 +449,46 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel
             st.load([&](int r, int which) {
                 const int key = key0 + r < p.Lk ? key0 + r : p.Lk - 1;
                 return which ? vb + key * p.sv.l : kb + key * p.sk.l;
-            }, p.Dk, p.Dv, p.sk.d, p.sv.d, p.vec, __builtin_amdgcn_readfirstlane(words[i]));
+            }, p.Dk, p.Dv, p.sk.d, p.sv.d, p.vec);
         };
         int i = next(0), buf = 0;
         if (i < wn) fetch(i);
         while (i < wn) {
-            st.store(Ks[buf], Vs[buf]);
-            __syncthreads();
             const uint32_t word = __builtin_amdgcn_readfirstlane(words[i]);
+            st.store(Ks[buf], Vs[buf], p.Dk, p.Dv, word);
+            __syncthreads();
             i = next(i + 1);
             if (i < wn) fetch(i);
             const T *ks = Ks[buf], *vs = Vs[buf];
             Acc s[NS];
 #pragma unroll
-            for (int u = 0; u < NS; u++) {
-                s[u] = 0;
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const V a = *(const V*)&ks[(u * M + c) * P + GN * t + h * N];
-#pragma unroll
-                    for (int e = 0; e < N; e++) s[u] = A::mfma(a[e], q[t][e], s[u]);
-                }
-            }
+            for (int u = 0; u < NS; u++) Ops::scores(s[u], ks + (u * M + c) * P + h * N, q);
             const T alpha = att_softmax<A, NS>(s, word, h, p.scale_base, m, l);
             if (__any(alpha != T(1))) {
 #pragma unroll
                 for (int d = 0; d < ND; d++) o[d] *= alpha;
             }
 #pragma unroll
-            for (int u = 0; u < NS; u++)
-#pragma unroll
-                for (int r = 0; r < A::R; r++)
-#pragma unroll
-                    for (int d = 0; d < ND; d++) o[d] = A::mfma(vs[(u * M + A::acc_row(r, h)) * P + d * M + c], s[u][r], o[d]);
+            for (int u = 0; u < NS; u++) Ops::outer(o, vs + Ops::E * c, u * A::R, h, s[u]);
             buf ^= 1;
         }
     }
     l = across_sum<A>(l);
-    if (live) att_store<A, ND>(p, o, [&](int i, int r) { return i * M + A::acc_row(r, h); }, head, b, hk, row, split, h, m, l);
+    if (live) att_store<Ops>(p, o, head, b, hk, row, split, h, m, l);
 }
 
 // Few rows (a decoding step): one wavefront takes 16 rows and a share of the keys, straight from memory into the operands' registers.
 // Bound by the bytes of the keys and values: 32 keys at width 64 are 2048 cycles of the matrix pipe and 16 KB, i.e. the pipes keep up with
 // three times the memory's rate.  A lane of value row `key` loads elements 16-byte-wise and uses element e of load g for
 // accumulator E g + e: accumulator i holds the elements E 16 g + E row + e of the result.
-template <class A, int DP>
+template <class A, int DP, bool WHOLE>
 __global__ __launch_bounds__(64) void attention_few_kernel(AttArgs<typename A::T> p) {
     using T = typename A::T;
     using V = typename Vec16<T>::type;
     using Acc = typename A::Acc;
     // (double precision at width 128: 16 keys a step, 32 do not fit the registers)
     constexpr int M = A::M, N = A::N, GN = A::G * N, NT = DP / GN, NS = sizeof(T) * DP > 512 ? 1 : 2, ND = DP / M, NG = ND / N, KEYS = NS * M;
-    static_assert(M == 16 && NG * N == ND, "whole loads");
+    static_assert(M == 16 && NG * N == ND && AttOps<A, DP>::E == N, "whole loads");
     uint32_t head, inner;
     att_place(blockIdx.x, p.blocks * p.splits, p.B * p.Hk, &head, &inner);
     const uint32_t block = inner / p.splits, split = inner - block * p.splits;
@@ -376,7 +499,7 @@ __global__ __launch_bounds__(64) void attention_few_kernel(AttArgs<typename A::T
     const T* qr = p.q + att_row(p, p.sq, b, hk, live ? row : 0);
     V q[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) q[t] = att_load<T>(qr, GN * t + h * N, p.Dk, p.sq.d, p.vec);
+    for (int t = 0; t < NT; t++) q[t] = att_piece<T, WHOLE>(qr, GN * t + h * N, p.Dk, p.sq.d, p.vec);
     Acc o[ND];
 #pragma unroll
     for (int i = 0; i < ND; i++) o[i] = 0;
@@ -385,7 +508,6 @@ __global__ __launch_bounds__(64) void attention_few_kernel(AttArgs<typename A::T
     const int t0 = split * p.split_tiles, t1 = tiles < (int)(t0 + p.split_tiles) ? tiles : (int)(t0 + p.split_tiles);
     const T* kb = p.k + b * p.sk.b + hk * p.sk.h;
     const T* vb = p.v + b * p.sv.b + hk * p.sv.h;
-    const bool whole = p.vec && p.Dk == DP && p.Dv == DP;
     uint32_t word = t0 < t1 ? (uint32_t)__ballot(att_key_on(p, b, t0 * kAttTile + (lane & 31))) : 0u;
     for (int t = t0; t < t1; t++) {
         const uint32_t now = word;
@@ -396,26 +518,26 @@ __global__ __launch_bounds__(64) void attention_few_kernel(AttArgs<typename A::T
             if (on == 0) continue;
             const int key0 = t * kAttTile + part * KEYS;
             V ka[NS][NT], va[NS][A::R][NG];
-            auto rows_of = [&](auto load) {
-#pragma unroll
-                for (int u = 0; u < NS; u++) {
-                    const int key = key0 + u * M + c;
-                    const T* kr = kb + (key < p.Lk ? key : p.Lk - 1) * p.sk.l;
-#pragma unroll
-                    for (int i = 0; i < NT; i++) ka[u][i] = load(kr, GN * i + h * N, p.Dk, p.sk.d);
-                }
-#pragma unroll
-                for (int u = 0; u < NS; u++)
-#pragma unroll
-                    for (int r = 0; r < A::R; r++) {
-                        const int key = key0 + u * M + A::acc_row(r, h);
-                        const T* vr = vb + (key < p.Lk ? key : p.Lk - 1) * p.sv.l;
-#pragma unroll
-                        for (int g = 0; g < NG; g++) va[u][r][g] = load(vr, (16 * g + c) * N, p.Dv, p.sv.d);
-                    }
+            auto load = [&](const T* base, int d, int D, int64_t sd) {   // (what lies beyond Dk meets zeros of the query, beyond Dv is not stored)
+                if constexpr (WHOLE) return *(const V*)(base + (d < D ? d : 0));
+                else return att_load<T>(base, d, D, sd, p.vec);
             };
-            if (whole) rows_of([](const T* base, int d, int, int64_t) { return *(const V*)(base + d); });
-            else rows_of([&](const T* base, int d, int D, int64_t sd) { return att_load<T>(base, d, D, sd, p.vec); });
+#pragma unroll
+            for (int u = 0; u < NS; u++) {
+                const int key = key0 + u * M + c;
+                const T* kr = kb + (key < p.Lk ? key : p.Lk - 1) * p.sk.l;
+#pragma unroll
+                for (int i = 0; i < NT; i++) ka[u][i] = load(kr, GN * i + h * N, p.Dk, p.sk.d);
+            }
+#pragma unroll
+            for (int u = 0; u < NS; u++)
+#pragma unroll
+                for (int r = 0; r < A::R; r++) {
+                    const int key = key0 + u * M + A::acc_row(r, h);
+                    const T* vr = vb + (key < p.Lk ? key : p.Lk - 1) * p.sv.l;
+#pragma unroll
+                    for (int g = 0; g < NG; g++) va[u][r][g] = load(vr, (16 * g + c) * N, p.Dv, p.sv.d);
+                }
             Acc s[NS];
 #pragma unroll
             for (int u = 0; u < NS; u++) {
@@ -449,7 +571,7 @@ __global__ __launch_bounds__(64) void attention_few_kernel(AttArgs<typename A::T
         word = (uint32_t)__ballot(ahead);
     }
     l = across_sum<A>(l);
-    if (live) att_store<A, ND>(p, o, [&](int i, int r) { return 16 * N * (i / N) + N * A::acc_row(r, h) + i % N; }, head, b, hk, row, split, h, m, l);
+    if (live) att_store<AttOps<A, DP>>(p, o, head, b, hk, row, split, h, m, l);   // (E = N there, too: the same elements in the same accumulators)
 }
 
 // Joins the shares of each row: a wavefront per row, first the shares' weights across its lanes, then lanes along the width.
@@ -521,12 +643,13 @@ template <class T, int DP> struct GradLds {
 };
 
 // dq: a wavefront owns M rows and walks the keys, as the forward pass does.
-template <class A, int DP>
+template <class A, int DP, bool WHOLE>
 __device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<typename A::T, DP>& lds, uint32_t at) {
     using T = typename A::T;
     using V = typename Vec16<T>::type;
     using Acc = typename A::Acc;
     constexpr int M = A::M, N = A::N, GN = A::G * N, NT = DP / GN, NS = kAttTile / M, ND = DP / M, P = kAttPitch<T, DP>, WAVES = kGradWaves;
+    using Ops = AttOps<A, DP>;
     uint32_t head, inner;
     att_place(at, p.blocks * p.splits, p.B * p.Hk, &head, &inner);
     const uint32_t block = inner / p.splits, split = inner - block * p.splits;
@@ -539,8 +662,8 @@ __device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<
     const T* gr = p.d_out + att_row(p, p.sdo, b, hk, live ? row : 0);
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-        q[t] = att_load<T>(qr, GN * t + h * N, p.Dk, p.sq.d, p.vec);
-        g[t] = att_load<T>(gr, GN * t + h * N, p.Dv, p.sdo.d, p.vec);
+        q[t] = att_piece<T, WHOLE>(qr, GN * t + h * N, p.Dk, p.sq.d, p.vec);
+        g[t] = att_piece<T, WHOLE>(gr, GN * t + h * N, p.Dv, p.sdo.d, p.vec);
     }
     const T lse = live ? att_lse<A>(p.lse[att_row(p, p.slse, b, hk, row)]) : (T)__builtin_inf();
     const T delta = live ? p.delta[(size_t)head * p.rows + row] : T(0);
@@ -551,7 +674,7 @@ __device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<
     const int t0 = split * p.split_tiles, t1 = tiles < (int)(t0 + p.split_tiles) ? tiles : (int)(t0 + p.split_tiles);
     const T* kb = p.k + b * p.sk.b + hk * p.sk.h;
     const T* vb = p.v + b * p.sv.b + hk * p.sv.h;
-    AttStage<T, DP, WAVES> st;
+    AttStage<T, DP, WAVES, WHOLE> st;
     for (int w0 = t0; w0 < t1; w0 += kAttWords) {
         const int wn = t1 - w0 < kAttWords ? t1 - w0 : kAttWords;
         __syncthreads();
@@ -566,30 +689,21 @@ __device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<
             st.load([&](int r, int which) {
                 const int key = key0 + r < p.Lk ? key0 + r : p.Lk - 1;
                 return which ? vb + key * p.sv.l : kb + key * p.sk.l;
-            }, p.Dk, p.Dv, p.sk.d, p.sv.d, p.vec, __builtin_amdgcn_readfirstlane(lds.words[i]));
+            }, p.Dk, p.Dv, p.sk.d, p.sv.d, p.vec);
         };
         int i = next(0), buf = 0;
         if (i < wn) fetch(i);
         while (i < wn) {
-            st.store(lds.a[buf], lds.b[buf]);
-            __syncthreads();
             const uint32_t word = __builtin_amdgcn_readfirstlane(lds.words[i]);
+            st.store(lds.a[buf], lds.b[buf], p.Dk, p.Dv, word);
+            __syncthreads();
             i = next(i + 1);
             if (i < wn) fetch(i);
             const T *ks = lds.a[buf], *vs = lds.b[buf];
 #pragma unroll
             for (int u = 0; u < NS; u++) {
-                Acc s = 0, dp = 0;
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const V a = *(const V*)&ks[(u * M + c) * P + GN * t + h * N];
-                    const V w = *(const V*)&vs[(u * M + c) * P + GN * t + h * N];
-#pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        s = A::mfma(a[e], q[t][e], s);
-                        dp = A::mfma(w[e], g[t][e], dp);
-                    }
-                }
+                Acc s, dp;
+                Ops::scores(s, ks + (u * M + c) * P + h * N, q, dp, vs + (u * M + c) * P + h * N, g);
 #pragma unroll
                 for (int r = 0; r < A::R; r++) s[r] = A::exp_(s[r] * p.scale_base - lse) * (dp[r] - delta) * p.scale;
                 if (word != ~0u) {
@@ -597,10 +711,7 @@ __device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<
                     for (int r = 0; r < A::R; r++)
                         if (!((word >> (u * M + A::acc_row(r, h))) & 1u)) s[r] = 0;
                 }
-#pragma unroll
-                for (int r = 0; r < A::R; r++)
-#pragma unroll
-                    for (int d = 0; d < ND; d++) dq[d] = A::mfma(ks[(u * M + A::acc_row(r, h)) * P + d * M + c], s[r], dq[d]);
+                Ops::outer(dq, ks + Ops::E * c, u * A::R, h, s);
             }
             buf ^= 1;
         }
@@ -615,22 +726,17 @@ __device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<
         o = p.part_dq + (((size_t)split * p.B * p.Hk + head) * p.rows + row) * p.Dk;
         sd = 1;
     }
-#pragma unroll
-    for (int i = 0; i < ND; i++)
-#pragma unroll
-        for (int r = 0; r < A::R; r++) {
-            const int d = i * M + A::acc_row(r, h);
-            if (d < p.Dk) o[d * sd] = dq[i][r];
-        }
+    Ops::put(o, sd, p.Dk, dq, T(1), h);
 }
 
 // dk and dv: a wavefront owns M keys and walks the rows of the group's query heads.
-template <class A, int DP>
+template <class A, int DP, bool WHOLE>
 __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds<typename A::T, DP>& lds, uint32_t at) {
     using T = typename A::T;
     using V = typename Vec16<T>::type;
     using Acc = typename A::Acc;
     constexpr int M = A::M, N = A::N, GN = A::G * N, NT = DP / GN, NS = kAttTile / M, ND = DP / M, P = kAttPitch<T, DP>, WAVES = kGradWaves;
+    using Ops = AttOps<A, DP>;
     uint32_t head, inner;
     att_place(at, p.kblocks * p.ksplits, p.B * p.Hk, &head, &inner);
     const uint32_t block = inner / p.ksplits, split = inner - block * p.ksplits;
@@ -644,10 +750,12 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
         const T* vr = p.v + b * p.sv.b + hk * p.sv.h + (in ? key : 0) * p.sv.l;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            k[t] = att_load<T>(kr, GN * t + h * N, p.Dk, p.sk.d, p.vec);
-            v[t] = att_load<T>(vr, GN * t + h * N, p.Dv, p.sv.d, p.vec);
-            if (!on) k[t] = v[t] = 0;
+            k[t] = att_piece<T, WHOLE>(kr, GN * t + h * N, p.Dk, p.sk.d, p.vec);
+            v[t] = att_piece<T, WHOLE>(vr, GN * t + h * N, p.Dv, p.sv.d, p.vec);
         }
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+            if (!on) k[t] = v[t] = 0;
     }
     Acc dk[ND], dv[ND];
 #pragma unroll
@@ -655,26 +763,28 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
     const int tiles = ((int)p.rows + kAttTile - 1) / kAttTile;
     const int t0 = split * p.ksplit_tiles, t1 = tiles < (int)(t0 + p.ksplit_tiles) ? tiles : (int)(t0 + p.ksplit_tiles);
     const bool any = __syncthreads_or((int)on);   // a block whose keys are all masked has nothing to add up
-    AttStage<T, DP, WAVES> st;
+    AttStage<T, DP, WAVES, WHOLE> st;
     T lse = 0, delta = 0;                          // of row threadIdx.x of the tile in flight
     auto fetch = [&](int t) {
-        const uint32_t r0 = (uint32_t)t * kAttTile, left = p.rows - r0;
+        const uint32_t r0 = (uint32_t)t * kAttTile;
         st.load([&](int r, int which) {
             const uint32_t at_row = r0 + r < p.rows ? r0 + r : p.rows - 1;
             return which ? p.d_out + att_row(p, p.sdo, b, hk, at_row) : p.q + att_row(p, p.sq, b, hk, at_row);
-        }, p.Dk, p.Dv, p.sq.d, p.sdo.d, p.vec, left >= 32 ? ~0u : (1u << left) - 1u);
+        }, p.Dk, p.Dv, p.sq.d, p.sdo.d, p.vec);
         if (threadIdx.x < kAttTile) {
             const uint32_t r = r0 + threadIdx.x;
-            lse = r < p.rows ? att_lse<A>(p.lse[att_row(p, p.slse, b, hk, r)]) : (T)__builtin_inf();
-            delta = r < p.rows ? p.delta[(size_t)head * p.rows + r] : T(0);
+            const uint32_t at_row = r < p.rows ? r : p.rows - 1;   // (rows beyond the last are zeros in the tile: what they get here adds nothing)
+            lse = p.lse[att_row(p, p.slse, b, hk, at_row)];         // as loaded: computing with it here would wait for the whole tile
+            delta = p.delta[(size_t)head * p.rows + at_row];
         }
     };
     int buf = 0;
     if (any && t0 < t1) fetch(t0);
     for (int t = t0; any && t < t1; t++) {
-        st.store(lds.a[buf], lds.b[buf]);
+        const uint32_t left = p.rows - (uint32_t)t * kAttTile;
+        st.store(lds.a[buf], lds.b[buf], p.Dk, p.Dv, left >= 32 ? ~0u : (1u << left) - 1u);
         if (threadIdx.x < kAttTile) {
-            lds.lse[buf][threadIdx.x] = lse;
+            lds.lse[buf][threadIdx.x] = t * kAttTile + threadIdx.x < p.rows ? att_lse<A>(lse) : (T)__builtin_inf();
             lds.delta[buf][threadIdx.x] = delta;
         }
         __syncthreads();
@@ -682,17 +792,8 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
         const T *qs = lds.a[buf], *gs = lds.b[buf];
 #pragma unroll
         for (int u = 0; u < NS; u++) {
-            Acc s = 0, dp = 0;
-#pragma unroll
-            for (int i = 0; i < NT; i++) {
-                const V a = *(const V*)&qs[(u * M + c) * P + GN * i + h * N];
-                const V w = *(const V*)&gs[(u * M + c) * P + GN * i + h * N];
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    s = A::mfma(a[e], k[i][e], s);
-                    dp = A::mfma(w[e], v[i][e], dp);
-                }
-            }
+            Acc s, dp;
+            Ops::scores(s, qs + (u * M + c) * P + h * N, k, dp, gs + (u * M + c) * P + h * N, v);
 #pragma unroll
             for (int r = 0; r < A::R; r++) {
                 const int i = u * M + A::acc_row(r, h);
@@ -700,14 +801,7 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
                 dp[r] = on ? pr * (dp[r] - lds.delta[buf][i]) * p.scale : T(0);
                 s[r] = pr;
             }
-#pragma unroll
-            for (int r = 0; r < A::R; r++)
-#pragma unroll
-                for (int i = 0; i < ND; i++) {
-                    const int at_lds = (u * M + A::acc_row(r, h)) * P + i * M + c;
-                    dv[i] = A::mfma(gs[at_lds], s[r], dv[i]);
-                    dk[i] = A::mfma(qs[at_lds], dp[r], dk[i]);
-                }
+            Ops::outer(dv, gs + Ops::E * c, s, dk, qs + Ops::E * c, dp, u * A::R, h);
         }
         buf ^= 1;
     }
@@ -725,23 +819,17 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
         ov = p.part_dv + at_row * p.Dv;
         sk = sv = 1;
     }
-#pragma unroll
-    for (int i = 0; i < ND; i++)
-#pragma unroll
-        for (int r = 0; r < A::R; r++) {
-            const int d = i * M + A::acc_row(r, h);
-            if (d < p.Dk) ok[d * sk] = dk[i][r];
-            if (d < p.Dv) ov[d * sv] = dv[i][r];
-        }
+    Ops::put(ok, sk, p.Dk, dk, T(1), h);
+    Ops::put(ov, sv, p.Dv, dv, T(1), h);
 }
 
 // Both halves of the backward pass in one launch: the workgroups of dk and dv first (they are the longer ones), then those of dq, so that
 // neither half leaves compute units idle while the other runs out.
-template <class A, int DP>
+template <class A, int DP, bool WHOLE>
 __global__ __launch_bounds__(64 * kGradWaves, DP <= 64 ? 2 : 1) void attention_grad_kernel(AttArgs<typename A::T> p, uint32_t kv_workgroups) {
     __shared__ __attribute__((aligned(16))) GradLds<typename A::T, DP> lds;
-    if (blockIdx.x < kv_workgroups) att_dkv<A, DP>(p, lds, blockIdx.x);
-    else att_dq<A, DP>(p, lds, blockIdx.x - kv_workgroups);
+    if (blockIdx.x < kv_workgroups) att_dkv<A, DP, WHOLE>(p, lds, blockIdx.x);
+    else att_dq<A, DP, WHOLE>(p, lds, blockIdx.x - kv_workgroups);
 }
 
 // Adds up the shares: workgroups [0, kv) take rows of dk and dv, the others rows of dq; a thread per element.
@@ -858,12 +946,16 @@ template <class T> int32_t attention_forward_impl(AttArgs<T>& p, void* scratch, 
     const dim3 grid(heads * p.blocks * p.splits);
     const int width = p.Dk > p.Dv ? p.Dk : p.Dv;
     if (pl.waves == 0) {
-        if (width <= 64) hipLaunchKernelGGL((attention_few_kernel<Few, 64>), grid, dim3(64), 0, s, p);
-        else hipLaunchKernelGGL((attention_few_kernel<Few, 128>), grid, dim3(64), 0, s, p);
+        if (width <= 64 && p.whole) hipLaunchKernelGGL((attention_few_kernel<Few, 64, true>), grid, dim3(64), 0, s, p);
+        else if (width <= 64) hipLaunchKernelGGL((attention_few_kernel<Few, 64, false>), grid, dim3(64), 0, s, p);
+        else if (p.whole) hipLaunchKernelGGL((attention_few_kernel<Few, 128, true>), grid, dim3(64), 0, s, p);
+        else hipLaunchKernelGGL((attention_few_kernel<Few, 128, false>), grid, dim3(64), 0, s, p);
     } else {
         att_widths<T>(width, [&](auto dp) {
-            if (pl.waves == 2) hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 2>), grid, dim3(128), 0, s, p);
-            else hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 4>), grid, dim3(256), 0, s, p);
+            if (pl.waves == 2 && p.whole) hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 2, true>), grid, dim3(128), 0, s, p);
+            else if (pl.waves == 2) hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 2, false>), grid, dim3(128), 0, s, p);
+            else if (p.whole) hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 4, true>), grid, dim3(256), 0, s, p);
+            else hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 4, false>), grid, dim3(256), 0, s, p);
         });
     }
     DNH_LAUNCH_CHECK();
@@ -898,7 +990,8 @@ template <class T> int32_t attention_backward_impl(AttArgs<T>& p, void* scratch,
     const uint32_t kv = p.dk ? (uint32_t)heads * p.kblocks * p.ksplits : 0, dq = p.dq ? (uint32_t)heads * p.blocks * p.splits : 0;
     if (kv + dq == 0) return DNH_OK;
     att_widths<T>(p.Dk > p.Dv ? p.Dk : p.Dv, [&](auto dp) {
-        hipLaunchKernelGGL((attention_grad_kernel<Tile, dp.value>), dim3(kv + dq), dim3(64 * kGradWaves), 0, s, p, kv);
+        if (p.whole) hipLaunchKernelGGL((attention_grad_kernel<Tile, dp.value, true>), dim3(kv + dq), dim3(64 * kGradWaves), 0, s, p, kv);
+        else hipLaunchKernelGGL((attention_grad_kernel<Tile, dp.value, false>), dim3(kv + dq), dim3(64 * kGradWaves), 0, s, p, kv);
     });
     DNH_LAUNCH_CHECK();
     const unsigned jkv = p.dk && p.ksplits > 1 ? cdiv(heads * p.Lk * (p.Dk + p.Dv), 256) : 0, jdq = p.dq && p.splits > 1 ? cdiv(heads * p.rows * p.Dk, 256) : 0;
