@@ -143,7 +143,7 @@ extern "C" int32_t dnh_cross_attention_scratch_bytes(int32_t dtype, int64_t batc
     const int64_t n = batch * kv_heads, rows = heads / kv_heads * queries;
     *bytes = 0;
     if (n == 0 || rows == 0) return DNH_OK;
-    const size_t f = dtype == DNH_F32 ? att_plan<float>(n, rows, keys, width).total : att_plan<double>(n, rows, keys, width).total;
+    const size_t f = dtype == DNH_F32 ? att_plan<float>(n, rows, keys, width, width).total : att_plan<double>(n, rows, keys, width, width).total;
     const size_t b = dtype == DNH_F32 ? att_grad_plan<float>(n, rows, keys, width, width).total : att_grad_plan<double>(n, rows, keys, width, width).total;
     *bytes = f > b ? f : b;
     return DNH_OK;

@@ -823,13 +823,15 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
     Ops::put(ov, sv, p.Dv, dv, T(1), h);
 }
 
-// Both halves of the backward pass in one launch: the workgroups of dk and dv first (they are the longer ones), then those of dq, so that
-// neither half leaves compute units idle while the other runs out.
+// Both halves of the backward pass in one launch, so that neither leaves compute units idle while the other runs out: `first` workgroups of
+// dq (dq_first) or of dk and dv, then those of the other.  The half with the longer walks goes first: what is left for the end is short.
 template <class A, int DP, bool WHOLE>
-__global__ __launch_bounds__(64 * kGradWaves, DP <= 64 ? 2 : 1) void attention_grad_kernel(AttArgs<typename A::T> p, uint32_t kv_workgroups) {
+__global__ __launch_bounds__(64 * kGradWaves, DP <= 64 ? 2 : 1) void attention_grad_kernel(AttArgs<typename A::T> p, uint32_t first, bool dq_first) {
     __shared__ __attribute__((aligned(16))) GradLds<typename A::T, DP> lds;
-    if (blockIdx.x < kv_workgroups) att_dkv<A, DP, WHOLE>(p, lds, blockIdx.x);
-    else att_dq<A, DP, WHOLE>(p, lds, blockIdx.x - kv_workgroups);
+    const bool front = blockIdx.x < first;
+    const uint32_t at = front ? blockIdx.x : blockIdx.x - first;
+    if (front == dq_first) att_dq<A, DP, WHOLE>(p, lds, at);
+    else att_dkv<A, DP, WHOLE>(p, lds, at);
 }
 
 // Adds up the shares: workgroups [0, kv) take rows of dk and dv, the others rows of dq; a thread per element.
@@ -872,14 +874,28 @@ inline void att_shares(int64_t workgroups, int64_t tiles, int64_t want, int64_t 
     *share_tiles = (uint32_t)each;
 }
 
+// Estimates in microseconds that choose the numbers of shares.  A product of a 32-row tile takes a wavefront DP x 32 cycles of its SIMD's
+// matrix pipe in either precision, at about 2.2 GHz; what else a tile costs it (softmax, staging, a barrier) about 1 us; starting and ending
+// a workgroup 4 us.  Up to padded width 64 two workgroups of four wavefronts fit a compute unit (they share the pipes), above one.
+// Measured with these against a fixed target of 256 workgroups: 80 row blocks at width 128 over 3000 keys 258 -> 199 us forward.
+inline int att_resident(int64_t width) { return width <= 64 ? 2 : 1; }
+inline double att_walk_us(int64_t width, int products, int64_t tiles) {
+    const double padded = (double)((width + 31) / 32 * 32);
+    return 4.0 + tiles * (products * padded * 0.0145 * att_resident(width) + 1.0);
+}
+// `n` workgroups of `each` us on `slots` places: what a place has to do on average, and half a walk for the uneven end
+inline double att_span_us(double n, double each, double slots) { return n <= slots ? each : n * each / slots + 0.5 * each; }
+inline double att_join_us(double bytes) { return bytes > 0 ? 5.0 + 2 * bytes / 4.0e6 : 0.0; }
+
 struct AttPlan {
     int waves;   // 0: the kernel for few rows
     uint32_t blocks, splits, split_tiles;
     size_t o_bytes, m_bytes, total;
 };
-template <class T> AttPlan att_plan(int64_t heads, int64_t rows, int64_t Lk, int64_t Dv) {
+template <class T> AttPlan att_plan(int64_t heads, int64_t rows, int64_t Lk, int64_t Dk, int64_t Dv) {
     constexpr int M = MmaOf<T>::Tile::M;
     AttPlan p;
+    const int64_t width = Dk > Dv ? Dk : Dv;
     const int64_t tiles = (Lk + kAttTile - 1) / kAttTile;
     if (rows <= kFewRows) {
         p.waves = 0;
@@ -888,7 +904,17 @@ template <class T> AttPlan att_plan(int64_t heads, int64_t rows, int64_t Lk, int
     } else {
         p.waves = rows <= 2 * M ? 2 : 4;
         p.blocks = cdiv(rows, (int64_t)p.waves * M);
-        att_shares(heads * p.blocks, tiles, 2 * kAttCUs * 4 / p.waves / 2, 64, &p.splits, &p.split_tiles);
+        const double slots = (double)kAttCUs * att_resident(width) * 4 / p.waves;
+        double best = 0;
+        for (int64_t n = 1; n <= 64 && (n == 1 || 2 * n <= tiles + 1); n++) {
+            const int64_t each = (tiles + n - 1) / n;
+            const double us = att_span_us((double)heads * p.blocks * n, att_walk_us(width, 2, each), slots) + att_join_us(n > 1 ? (double)heads * rows * n * Dv * sizeof(T) : 0.0);
+            if (n > 1 && us >= best) continue;
+            best = us;
+            p.split_tiles = (uint32_t)(each < 1 ? 1 : each);
+            p.splits = cdiv(tiles, p.split_tiles);
+            if (p.splits < 1) p.splits = 1;
+        }
     }
     const size_t parts = (size_t)heads * rows * p.splits;
     p.o_bytes = up256(parts * Dv * sizeof(T));
@@ -906,8 +932,26 @@ template <class T> AttGradPlan att_grad_plan(int64_t heads, int64_t rows, int64_
     AttGradPlan p;
     p.blocks = cdiv(rows, kGradWaves * M);
     p.kblocks = cdiv(Lk, kGradWaves * M);
-    att_shares(heads * p.blocks, (Lk + kAttTile - 1) / kAttTile, kAttCUs, 64, &p.splits, &p.split_tiles);
-    att_shares(heads * p.kblocks, (rows + kAttTile - 1) / kAttTile, kAttCUs, 64, &p.ksplits, &p.ksplit_tiles);
+    // both numbers of shares at once: the halves run side by side
+    const int64_t width = Dk > Dv ? Dk : Dv, tk = (Lk + kAttTile - 1) / kAttTile, tr = (rows + kAttTile - 1) / kAttTile;
+    const double slots = (double)kAttCUs * att_resident(width), qn = (double)heads * p.blocks, kn = (double)heads * p.kblocks;
+    double best = 0;
+    for (int64_t n = 1; n <= 64 && (n == 1 || 2 * n <= tk + 1); n = n < 8 ? n + 1 : n + n / 4)
+        for (int64_t k = 1; k <= 64 && (k == 1 || 2 * k <= tr + 1); k = k < 8 ? k + 1 : k + k / 4) {
+            const int64_t eq = (tk + n - 1) / n, ek = (tr + k - 1) / k;
+            const double uq = att_walk_us(width, 3, eq), uk = att_walk_us(width, 4, ek), longest = uq > uk ? uq : uk;
+            const double even = (qn * n * uq + kn * k * uk) / slots + 0.5 * (uq < uk ? uq : uk);
+            const double bytes = (n > 1 ? (double)heads * rows * Dk * n : 0.0) + (k > 1 ? (double)heads * Lk * (Dk + Dv) * k : 0.0);
+            const double us = (qn * n + kn * k <= slots || even < longest ? longest : even) + att_join_us(bytes * sizeof(T));
+            if ((n > 1 || k > 1) && us >= best) continue;
+            best = us;
+            p.split_tiles = (uint32_t)(eq < 1 ? 1 : eq);
+            p.splits = cdiv(tk, p.split_tiles);
+            if (p.splits < 1) p.splits = 1;
+            p.ksplit_tiles = (uint32_t)(ek < 1 ? 1 : ek);
+            p.ksplits = cdiv(tr, p.ksplit_tiles);
+            if (p.ksplits < 1) p.ksplits = 1;
+        }
     p.delta_bytes = up256((size_t)heads * rows * sizeof(T));
     p.dq_bytes = p.splits > 1 ? up256((size_t)p.splits * heads * rows * Dk * sizeof(T)) : 0;
     p.dk_bytes = p.ksplits > 1 ? up256((size_t)p.ksplits * heads * Lk * Dk * sizeof(T)) : 0;
@@ -933,7 +977,7 @@ template <class T> int32_t attention_forward_impl(AttArgs<T>& p, void* scratch, 
     using Tile = typename MmaOf<T>::Tile;
     using Few = typename MmaOf<T>::Few;
     const uint32_t heads = (uint32_t)(p.B * p.Hk);
-    const AttPlan pl = att_plan<T>(heads, p.rows, p.Lk, p.Dv);
+    const AttPlan pl = att_plan<T>(heads, p.rows, p.Lk, p.Dk, p.Dv);
     p.blocks = pl.blocks;
     p.splits = pl.splits;
     p.split_tiles = pl.split_tiles;
@@ -989,9 +1033,12 @@ template <class T> int32_t attention_backward_impl(AttArgs<T>& p, void* scratch,
     }
     const uint32_t kv = p.dk ? (uint32_t)heads * p.kblocks * p.ksplits : 0, dq = p.dq ? (uint32_t)heads * p.blocks * p.splits : 0;
     if (kv + dq == 0) return DNH_OK;
+    // a tile costs three products in dq, four in dk and dv
+    const bool dq_first = 3 * (int64_t)p.split_tiles >= 4 * (int64_t)p.ksplit_tiles;
+    const uint32_t first = dq_first ? dq : kv;
     att_widths<T>(p.Dk > p.Dv ? p.Dk : p.Dv, [&](auto dp) {
-        if (p.whole) hipLaunchKernelGGL((attention_grad_kernel<Tile, dp.value, true>), dim3(kv + dq), dim3(64 * kGradWaves), 0, s, p, kv);
-        else hipLaunchKernelGGL((attention_grad_kernel<Tile, dp.value, false>), dim3(kv + dq), dim3(64 * kGradWaves), 0, s, p, kv);
+        if (p.whole) hipLaunchKernelGGL((attention_grad_kernel<Tile, dp.value, true>), dim3(kv + dq), dim3(64 * kGradWaves), 0, s, p, first, dq_first);
+        else hipLaunchKernelGGL((attention_grad_kernel<Tile, dp.value, false>), dim3(kv + dq), dim3(64 * kGradWaves), 0, s, p, first, dq_first);
     });
     DNH_LAUNCH_CHECK();
     const unsigned jkv = p.dk && p.ksplits > 1 ? cdiv(heads * p.Lk * (p.Dk + p.Dv), 256) : 0, jdq = p.dq && p.splits > 1 ? cdiv(heads * p.rows * p.Dk, 256) : 0;
