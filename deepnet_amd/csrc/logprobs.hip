@@ -19,7 +19,7 @@ namespace {
 constexpr int kBlock = 256, kWaves = kBlock / 64;
 constexpr int kMaxTop = 64;                     // one alternative per lane of a wavefront
 constexpr uint32_t kNoIndex = 0xFFFFFFFFu;
-constexpr int kSlice = 2048;                    // fewest elements of a row that a workgroup takes when a row is shared
+constexpr int kSlice = 4096;                    // fewest elements of a row that a workgroup takes when a row is shared
 
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896340736f); }
 __device__ __forceinline__ double exp_of(double d) { return exp(d); }
@@ -54,14 +54,46 @@ __device__ __forceinline__ Stats wave_merge(Stats x) {
 // ---- the best K of a stream, one per lane in descending order ---------------------------------------------------------------------
 template <class T> __device__ __forceinline__ bool better(T v, uint32_t i, T w, uint32_t j) { return v > w || (v == w && i < j); }
 
+// Lane moves on 32-bit words, element-wise for wider types: no LDS round trip, which a cross-lane shuffle would take.
+template <class X> __device__ __forceinline__ X read_lane(X x, int lane) {   // lane: the same for the whole wavefront
+    int w[sizeof(X) / 4];
+    __builtin_memcpy(w, &x, sizeof(X));
+#pragma unroll
+    for (int k = 0; k < (int)(sizeof(X) / 4); k++) w[k] = __builtin_amdgcn_readlane(w[k], lane);
+    __builtin_memcpy(&x, w, sizeof(X));
+    return x;
+}
+template <class X> __device__ __forceinline__ X from_lane_below(X x) {       // lane l gets lane l - 1's, lane 0 keeps its own
+    int w[sizeof(X) / 4];
+    __builtin_memcpy(w, &x, sizeof(X));
+#pragma unroll
+    for (int k = 0; k < (int)(sizeof(X) / 4); k++) w[k] = __builtin_amdgcn_update_dpp(w[k], w[k], 0x138, 0xf, 0xf, false);   // wave_shr:1
+    __builtin_memcpy(&x, w, sizeof(X));
+    return x;
+}
+
+// Where a wavefront spreads some lanes' elements over all lanes (LDS accesses of one wavefront are served in order).
+template <class T> struct Spread {
+    T x[64];
+    uint32_t first[64], taken[64];
+};
+
 template <class T> struct TopList {
     T v;             // the lane-th best so far
     uint32_t i;      // kNoIndex: none yet
     T floor_v;       // the K-th best
     uint32_t floor_i;
     __device__ __forceinline__ void clear() {
-        v = floor_v = neg_inf<T>();
-        i = floor_i = kNoIndex;
+        v = neg_inf<T>();
+        i = kNoIndex;
+        // The floor lives in scalar registers, and a double there must not be a constant the compiler knows: it then writes -inf with one
+        // 64-bit scalar move, whose literal has only 32 bits (ROCm 7.2: the register pair gets 0.0).
+        int w[sizeof(T) / 4];
+        __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+        for (int k = 0; k < (int)(sizeof(T) / 4); k++) asm volatile("" : "+s"(w[k]));
+        __builtin_memcpy(&floor_v, w, sizeof(T));
+        floor_i = kNoIndex;
     }
     // every lane offers one element (`in`: it has one); NaN is never better than anything
     __device__ __forceinline__ void offer(T x, uint32_t j, bool in, int K) {
@@ -69,22 +101,89 @@ template <class T> struct TopList {
         const int lane = threadIdx.x & 63;
         while (m) {
             const int src = __builtin_ctzll(m);
-            m &= m - 1;
-            const T cv = __shfl(x, src);
-            const uint32_t ci = __shfl(j, src);
-            if (!better(cv, ci, floor_v, floor_i)) continue;
+            const T cv = read_lane(x, src);
+            const uint32_t ci = read_lane(j, src);
             const int at = __popcll(__ballot(better(v, i, cv, ci)));
-            const T pv = __shfl_up(v, 1);
-            const uint32_t pi = __shfl_up(i, 1);
-            if (lane > at) {
-                v = pv;
-                i = pi;
-            } else if (lane == at) {
-                v = cv;
-                i = ci;
+            const T pv = from_lane_below(v);
+            const uint32_t pi = from_lane_below(i);
+            v = lane > at ? pv : lane == at ? cv : v;
+            i = lane > at ? pi : lane == at ? ci : i;
+            floor_v = read_lane(v, K - 1);
+            floor_i = read_lane(i, K - 1);
+            // the floor has risen: those still waiting have to pass it anew
+            m &= m - 1;
+            m &= __ballot(better(x, j, floor_v, floor_i));
+        }
+    }
+    // joins another list of the same order.  Position by position the better one of this list and the other one reversed are the best
+    // 64 of both, descending and then ascending or the other way round; six exchanges sort them.
+    __device__ __forceinline__ void join(T ov, uint32_t oi, int K) {
+        const int lane = threadIdx.x & 63;
+        const T rv = __shfl(ov, 63 - lane);
+        const uint32_t ri = __shfl(oi, 63 - lane);
+        if (better(rv, ri, v, i)) {
+            v = rv;
+            i = ri;
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) exchange(v, i, d, (lane & d) == 0);
+        floor_v = read_lane(v, K - 1);
+        floor_i = read_lane(i, K - 1);
+    }
+    // one step of a sorting network: of lanes that differ in bit d, those with `keep` keep the better element
+    static __device__ __forceinline__ void exchange(T& v, uint32_t& i, int d, bool keep) {
+        const T pv = __shfl_xor(v, d);
+        const uint32_t pi = __shfl_xor(i, d);
+        if (better(pv, pi, v, i) == keep) {
+            v = pv;
+            i = pi;
+        }
+    }
+    // C elements of every lane, element c with index first + step(c) (ascending), those from index `end` on missing; big: the largest of them.
+    // When many lanes hold something for the list, as at the start of a row, the lanes' largest elements are sorted and joined at once; the
+    // K-th of them is then a floor that few others pass.  Then, 64 / C at a time, the lanes whose largest element reaches the floor spread
+    // their elements over the wavefront, and those above the floor are inserted one by one.
+    template <int C, class Step>
+    __device__ __forceinline__ void offer_all(const T (&x)[C], T big, uint32_t first, Step step, uint32_t end, int K, Spread<T>& sp) {
+        unsigned long long m = __ballot(big >= floor_v);
+        if (m == 0) return;
+        const int lane = threadIdx.x & 63;
+        uint32_t taken = kNoIndex;
+        if (__popcll(m) > 8) {
+            T bv = x[0];
+            uint32_t bi = first + step(0);
+#pragma unroll
+            for (int c = 1; c < C; c++)
+                if (x[c] > bv || bv != bv) {
+                    bv = x[c];
+                    bi = first + step(c);
+                }
+            if (bv != bv || bi >= end) {                 // a lane of NaNs, or of missing elements (-inf), has nothing to offer
+                bv = neg_inf<T>();
+                bi = kNoIndex;
             }
-            floor_v = __shfl(v, K - 1);
-            floor_i = __shfl(i, K - 1);
+            taken = bi;
+#pragma unroll
+            for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+                for (int d = k >> 1; d; d >>= 1) exchange(bv, bi, d, ((lane & d) == 0) == ((lane & k) == 0));
+            join(bv, bi, K);
+            m = __ballot(big >= floor_v);
+        }
+        constexpr int L = 64 / C;                        // lanes that spread at a time
+        while (m) {
+            const int rank = __popcll(m & ((1ull << lane) - 1ull));
+            if (((m >> lane) & 1ull) && rank < L) {
+#pragma unroll
+                for (int c = 0; c < C; c++) sp.x[rank * C + c] = x[c];
+                sp.first[rank] = first;
+                sp.taken[rank] = taken;
+            }
+            const uint32_t j = sp.first[lane / C] + step(lane % C);
+            offer(sp.x[lane], j, lane / C < __popcll(m) && j < end && j != sp.taken[lane / C], K);
+#pragma unroll
+            for (int k = 0; k < L; k++) m &= m - 1;      // (0 stays 0)
+            m &= __ballot(big >= floor_v);
         }
     }
 };
@@ -133,10 +232,60 @@ template <class T> __device__ __forceinline__ void take(T x, T m, double& s, dou
     s += (double)e;
     a += (double)(e * entropy_factor(d));
 }
+// the larger one; of a number and a NaN the number
+__device__ __forceinline__ float larger(float x, float y) {
+    float r;
+    // (fmaxf first quiets both operands: three instructions.  The operands must not come straight from a transcendental instruction, whose
+    // result the compiler separates from its user by a wait state only where it knows the user.)
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
+    return r;
+}
+__device__ __forceinline__ double larger(double x, double y) { return y > x || x != x ? y : x; }
+
+// U x N elements at once.  Single precision is bound by instructions if every term goes to double precision by itself (28 cycles of 4 per
+// element, 155 us for 4096 rows of 50 048, against 126 us for the bytes), so groups of U x N are added up in 32 bits first, five roundings
+// deep.  That would lose the rest beside a dominant logit, whose term is exactly 1: the ones are kept out of the sum (v_fract_f32 turns 1
+// into 0 and leaves what is below 1) and counted by the difference of the sums with and without them, which is a whole number
+// up to a rounding.
+template <int U, int N> __device__ __forceinline__ void take_all(const float (&x)[U][N], float m, double& s, double& a) {
+    float below[N], all[N], ed[N];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const float d = x[u][e] - m, t = exp_of(d), f = larger(d, -1.0e4f);   // (as entropy_factor)
+            below[e] = u ? below[e] + __builtin_amdgcn_fractf(t) : __builtin_amdgcn_fractf(t);
+            all[e] = u ? all[e] + t : t;
+            ed[e] = u ? __builtin_fmaf(t, f, ed[e]) : t * f;
+        }
+#pragma unroll
+    for (int w = 1; w < N; w <<= 1)
+#pragma unroll
+        for (int e = 0; e + w < N; e += 2 * w) {
+            below[e] += below[e + w];
+            all[e] += all[e + w];
+            ed[e] += ed[e + w];
+        }
+    s += (double)below[0] + (double)__builtin_rintf(all[0] - below[0]);
+    a += (double)ed[0];
+}
+template <int U, int N> __device__ __forceinline__ void take_all(const double (&x)[U][N], double m, double& s, double& a) {
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < N; e++) take(x[u][e], m, s, a);
+}
+// e^d for the sums' rescaling.  Single precision: the fraction of the exponent on the fast instruction (2 u), the whole part exactly; the
+// library's double-precision exponential would keep 20 registers of constants alive through the loop.
+__device__ __forceinline__ double shrink(double d, float) {
+    const double t = d * 1.44269504088896340736, n = __builtin_rint(t);
+    return ldexp((double)__builtin_amdgcn_exp2f((float)(t - n)), (int)n);
+}
+__device__ __forceinline__ double shrink(double d, double) { return exp(d); }
 
 // A workgroup takes elements [j0, j1) of a row.  With one workgroup per row it writes the results, else its statistics and list.
 template <class T, bool VEC, bool TOP>
-__global__ __launch_bounds__(kBlock) void log_probs_kernel(LogProbArgs<T> p, uint32_t splits, uint32_t slice, Stats* __restrict__ part_st, T* __restrict__ part_v,
+__global__ __launch_bounds__(kBlock, TOP ? 5 : 1) void log_probs_kernel(LogProbArgs<T> p, uint32_t splits, uint32_t slice, Stats* __restrict__ part_st, T* __restrict__ part_v,
                                                            uint32_t* __restrict__ part_i) {
     constexpr int N = VEC ? kVecN<T> : 1, U = 4;
     using V = typename Vec16<T>::type;
@@ -146,69 +295,75 @@ __global__ __launch_bounds__(kBlock) void log_probs_kernel(LogProbArgs<T> p, uin
     row_offsets(p.rp, row, off);
     const T* x = p.x + off[0];
     const int64_t j0 = (int64_t)split * slice, j1 = p.vocab - j0 < slice ? p.vocab : j0 + slice;
+    // the wavefront's maximum, and each lane's sums relative to it: with one maximum for all lanes, sums are rescaled (a double-precision
+    // exponential) about three times a row instead of in nearly every step, and lanes are joined by additions
     T m = neg_inf<T>();
     double s = 0, a = 0;
+    __shared__ Spread<T> spread[TOP ? kWaves : 1];
     TopList<T> top;
     top.clear();
-    auto raise = [&](T to) {   // a new maximum of this thread: rescale what it has
-        if (to > m) {
-            if (s != 0.0) {
-                const double d = entropy_factor((double)m - (double)to), e = exp(d);
-                a = e * (a + s * d);
-                s *= e;
-            }
-            m = to;
-        }
-    };
-    int64_t j = j0;
-    for (; j + (int64_t)U * kBlock * N <= j1; j += (int64_t)U * kBlock * N) {
+    for (int64_t j = j0; j < j1; j += U * kBlock * N) {
         T v[U][N];
+        const T* xs = x + j * p.xd;                                                 // the same for the whole workgroup
+        const int mine = (int)threadIdx.x * N, left = j1 - j < U * kBlock * N ? (int)(j1 - j) : U * kBlock * N;
+        if (left == U * kBlock * N) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t at = j + ((int64_t)u * kBlock + threadIdx.x) * N;
-            if constexpr (VEC) {
-                const V w = *(const V*)(x + at);
+            for (int u = 0; u < U; u++) {
+                if constexpr (VEC) {
+                    const V w = __builtin_nontemporal_load((const V*)(xs + (mine + u * kBlock * N)));
 #pragma unroll
-                for (int e = 0; e < N; e++) v[u][e] = w[e];
-            } else {
-                v[u][0] = x[at * p.xd];
+                    for (int e = 0; e < N; e++) v[u][e] = w[e];
+                } else {
+                    v[u][0] = xs[(mine + u * kBlock) * p.xd];
+                }
+            }
+        } else {
+            // (a missing element has probability 0)
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int at = mine + u * kBlock * N;
+                if (VEC && at + N <= left) {
+                    const V w = *(const V*)(xs + at);
+#pragma unroll
+                    for (int e = 0; e < N; e++) v[u][e] = w[e % kVecN<T>];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; e++) v[u][e] = at + e < left ? xs[VEC ? (int64_t)(at + e) : (at + e) * p.xd] : neg_inf<T>();
+                }
             }
         }
         T big = v[0][0];
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int e = 0; e < N; e++) big = v[u][e] > big || big != big ? v[u][e] : big;
-        raise(big);
-        const T mm = m == neg_inf<T>() ? T(0) : m;
+            for (int e = 0; e < N; e++) big = larger(big, v[u][e]);
+        if (__ballot(big > m)) {
+            T to = big > m ? big : m;
 #pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int e = 0; e < N; e++) take(v[u][e], mm, s, a);
+            for (int d = 1; d < 64; d <<= 1) to = larger(to, __shfl_xor(to, d));
+            const double d = entropy_factor((double)m - (double)to), e = shrink(d, T());   // (m = -inf: the sums are still zero)
+            a = e * (a + s * d);
+            s *= e;
+            m = to;
+        }
+        take_all(v, m == neg_inf<T>() ? T(0) : m, s, a);
         if constexpr (TOP) {
-            if (__ballot(big >= top.floor_v)) {
+            T flat[U * N];
 #pragma unroll
-                for (int u = 0; u < U; u++)
-#pragma unroll
-                    for (int e = 0; e < N; e++) top.offer(v[u][e], (uint32_t)(j + ((int64_t)u * kBlock + threadIdx.x) * N + e), true, p.K);
-            }
+            for (int k = 0; k < U * N; k++) flat[k] = v[k / N][k % N];
+            top.offer_all(flat, big, (uint32_t)j + (uint32_t)mine, [](int k) { return (uint32_t)(k / N * kBlock * N + k % N); }, (uint32_t)j1, p.K, spread[wave]);
         }
-    }
-    for (; j < j1; j += kBlock) {
-        const int64_t at = j + threadIdx.x;
-        const bool in = at < j1;
-        const T v = in ? x[at * p.xd] : neg_inf<T>();
-        if (in) {
-            raise(v);
-            take(v, m == neg_inf<T>() ? T(0) : m, s, a);
-        }
-        if constexpr (TOP) top.offer(v, (uint32_t)at, in, p.K);
     }
     // the wavefronts' parts meet in LDS; the first wavefront joins them
     __shared__ Stats wst[kWaves];
     __shared__ T wv[kWaves][kMaxTop];
     __shared__ uint32_t wi[kWaves][kMaxTop];
-    const Stats mine = wave_merge(Stats{(double)m, s, a});
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        s += __shfl_xor(s, d);
+        a += __shfl_xor(a, d);
+    }
+    const Stats mine{(double)m, s, a};
     if (lane == 0) wst[wave] = mine;
     if constexpr (TOP) {
         wv[wave][lane] = top.v;
@@ -219,7 +374,7 @@ __global__ __launch_bounds__(kBlock) void log_probs_kernel(LogProbArgs<T> p, uin
     Stats all = mine;
     for (int w = 1; w < kWaves; w++) {
         all = merge(all, wst[w]);
-        if constexpr (TOP) top.offer(wv[w][lane], wi[w][lane], lane < p.K && wi[w][lane] != kNoIndex, p.K);
+        if constexpr (TOP) top.join(wv[w][lane], wi[w][lane], p.K);
     }
     if (splits == 1) {
         finish_row(p, row, all, top.v, top.i);
@@ -232,27 +387,36 @@ __global__ __launch_bounds__(kBlock) void log_probs_kernel(LogProbArgs<T> p, uin
     }
 }
 
-// Joins the parts of a shared row, one wavefront per row.
+// Joins the parts of a shared row: the wavefronts of a workgroup take parts in turn, then each other's lists two by two.
+constexpr int kJoinWaves = 16;
 template <class T>
-__global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbArgs<T> p, uint32_t splits, const Stats* __restrict__ part_st, const T* __restrict__ part_v,
-                                                            const uint32_t* __restrict__ part_i) {
+__global__ __launch_bounds__(64 * kJoinWaves) void log_probs_join_kernel(LogProbArgs<T> p, uint32_t splits, const Stats* __restrict__ part_st,
+                                                                         const T* __restrict__ part_v, const uint32_t* __restrict__ part_i) {
+    __shared__ T wv[kJoinWaves][kMaxTop];
+    __shared__ uint32_t wi[kJoinWaves][kMaxTop];
     const uint32_t row = blockIdx.x;
-    const int lane = threadIdx.x;
-    Stats st = no_stats();
-    for (uint32_t k = lane; k < splits; k += 64) st = merge(st, part_st[(size_t)row * splits + k]);
-    st = wave_merge(st);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool mine = lane < p.K;
     TopList<T> top;
     top.clear();
     if (p.K > 0) {
-        const uint32_t n = splits * p.K;
-        for (uint32_t k = 0; k < n; k += 64) {
-            const bool in = k + lane < n;
-            const size_t at = (size_t)row * n + (in ? k + lane : 0);
-            const T v = part_v[at];
-            const uint32_t i = part_i[at];
-            top.offer(v, i, in && i != kNoIndex, p.K);
+        for (uint32_t k = wave; k < splits; k += kJoinWaves) {
+            const size_t at = ((size_t)row * splits + k) * p.K + lane;
+            top.join(mine ? part_v[at] : neg_inf<T>(), mine ? part_i[at] : kNoIndex, p.K);
+        }
+        for (int half = kJoinWaves / 2; half; half >>= 1) {
+            if (wave >= half && wave < 2 * half) {
+                wv[wave][lane] = top.v;
+                wi[wave][lane] = top.i;
+            }
+            __syncthreads();
+            if (wave < half) top.join(wv[wave + half][lane], wi[wave + half][lane], p.K);
         }
     }
+    if (wave != 0) return;
+    Stats st = no_stats();
+    for (uint32_t k = lane; k < splits; k += 64) st = merge(st, part_st[(size_t)row * splits + k]);
+    st = wave_merge(st);
     finish_row(p, row, st, top.v, top.i);
 }
 
@@ -321,7 +485,7 @@ int32_t log_probs(const DnhTensor* log_probs, const DnhTensor* lse, const DnhTen
     else hipLaunchKernelGGL((log_probs_kernel<T, false, false>), grid, block, 0, s, p, pp.splits, pp.slice, st, pv, pi);
     DNH_LAUNCH_CHECK();
     if (pp.splits > 1) {
-        hipLaunchKernelGGL((log_probs_join_kernel<T>), dim3(rows), dim3(64), 0, s, p, pp.splits, (const Stats*)st, (const T*)pv, (const uint32_t*)pi);
+        hipLaunchKernelGGL((log_probs_join_kernel<T>), dim3(rows), dim3(K ? 64 * kJoinWaves : 64), 0, s, p, pp.splits, (const Stats*)st, (const T*)pv, (const uint32_t*)pi);
         DNH_LAUNCH_CHECK();
     }
     return DNH_OK;
