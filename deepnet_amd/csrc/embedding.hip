@@ -83,11 +83,12 @@ int32_t launch_embedding(const DnhTensor* t, const DnhTensor* table, const DnhTe
 // all others, where nothing reads it.  Ranks come from ballots: lanes of a wavefront that share a digit find each other with one ballot
 // per digit bit; each wavefront counts its own digits in LDS while it walks its part of the tile in order.
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kMaxDigitBits = 9, kMaxDigits = 1 << kMaxDigitBits;
+constexpr int kMinDigitBits = 6, kMaxDigitBits = 9, kMaxDigits = 1 << kMaxDigitBits;
 constexpr uint32_t kSmallSort = 8192;    // tokens that one workgroup sorts in LDS, in one launch
-constexpr uint32_t kSortTile = 4096;     // tokens of a workgroup's step in the passes through memory
+constexpr uint32_t kSortTile = 1024;     // tokens of a workgroup's step in the passes through memory: one a thread, as its stores scatter over
+                                         // as many cache lines and a compute unit serves one line a cycle (4096: 15 us a pass instead of 9)
 constexpr int64_t kMaxGradTokens = (int64_t)1 << 27;   // keeps every grid of the gradient below 2^32 threads
-constexpr uint32_t kMaxChunks = 512;     // workgroups of such a pass: every one of them adds up the counts of all
+constexpr uint32_t kMaxChunks = 128;     // workgroups of such a pass: every one of them adds up the counts of all
 
 struct TokenSource {
     const int64_t* tokens;
@@ -104,11 +105,15 @@ __device__ __forceinline__ uint32_t token_key(const TokenSource& s, uint32_t i) 
     return s.vocab;
 }
 
+// Counters of (digit, wavefront), a digit's 16 side by side in 17 words: lanes of a wavefront with different digits meet different banks.
+constexpr int kCounters = kMaxDigits * (kSortWaves + 1);
+__device__ __forceinline__ int counter(uint32_t digit, int wave) { return (int)digit * (kSortWaves + 1) + wave; }
+
 // Rank of each of the thread's E keys (key e of lane l of wave w stands at w * 64 E + 64 e + l) among the wavefront's keys of the same
-// digit, and the wavefront's counts per digit in cnt[digit].
+// digit; the wavefront's counts per digit are left in cnt.
 template <int E>
 __device__ __forceinline__ void wave_ranks(const uint32_t (&digit)[E], const bool (&live)[E], int bits, uint32_t* cnt, uint32_t (&rank)[E]) {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int e = 0; e < E; e++) {
         unsigned long long peers = __ballot(live[e]);
@@ -119,15 +124,15 @@ __device__ __forceinline__ void wave_ranks(const uint32_t (&digit)[E], const boo
         }
         const uint32_t before = (uint32_t)__popcll(peers & ((1ull << lane) - 1ull));
         // LDS accesses of one wavefront are served in order: every lane reads the count, then the first of each group raises it
-        const uint32_t old = live[e] ? __hip_atomic_load(&cnt[digit[e]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) : 0u;
+        const int at = counter(digit[e], wave);
+        const uint32_t old = live[e] ? __hip_atomic_load(&cnt[at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) : 0u;
         rank[e] = old + before;
-        if (live[e] && before == 0)
-            __hip_atomic_store(&cnt[digit[e]], old + (uint32_t)__popcll(peers), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (live[e] && before == 0) __hip_atomic_store(&cnt[at], old + (uint32_t)__popcll(peers), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
 }
 
-// Exclusive scan of one value per thread over the first kMaxDigits threads; every thread of the workgroup calls it.
-__device__ __forceinline__ uint32_t digit_scan(uint32_t v, uint32_t* wave_sum) {
+// Exclusive scan of one value per thread; every thread of the workgroup calls it.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* wave_sum) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t x = v;
 #pragma unroll
@@ -137,10 +142,28 @@ __device__ __forceinline__ uint32_t digit_scan(uint32_t v, uint32_t* wave_sum) {
     }
     if (lane == 63) wave_sum[wave] = x;
     __syncthreads();
-    uint32_t base = 0;
-    for (int w = 0; w < wave; w++) base += wave_sum[w];
+    uint32_t base = lane < wave ? wave_sum[lane] : 0u;   // (16 wavefronts: the sums before this one lie in its first lanes)
+#pragma unroll
+    for (int d = 1; d < kSortWaves; d <<= 1) base += __shfl_xor(base, d);
+    base = __shfl(base, 0);
     __syncthreads();
     return base + x - v;
+}
+
+// Turns the counters into where each (digit, wavefront) starts in the sorted tile: an exclusive scan in that order, digits / 64 counters
+// (all of one digit) a thread.  Every thread of the workgroup calls it, with the counters complete; it ends with a barrier.
+__device__ __forceinline__ void scan_counters(uint32_t* cnt, int bits, uint32_t* wave_sum) {
+    const int per = (1 << bits) / 64;
+    const int at = counter(threadIdx.x * per / kSortWaves, threadIdx.x * per % kSortWaves);
+    uint32_t sum = 0;
+    for (int k = 0; k < per; k++) sum += cnt[at + k];
+    uint32_t run = block_scan(sum, wave_sum);
+    for (int k = 0; k < per; k++) {
+        const uint32_t c = cnt[at + k];
+        cnt[at + k] = run;
+        run += c;
+    }
+    __syncthreads();
 }
 
 // Fills rows [row0, row1) of a target with zeros; workgroup `wg` of `wgs`.
@@ -164,18 +187,17 @@ __device__ __forceinline__ void zero_rows(const ZeroRows<T>& z, uint32_t wg, uin
         for (int64_t c = threadIdx.x; c < z.width; c += threads) z.t[r * z.row_stride + c * z.d_stride] = T(0);
 }
 
-// Workgroup 0 sorts up to kSmallSort tokens in LDS; the others clear the target meanwhile.
-template <class T>
+// Workgroup 0 sorts up to 1024 E tokens in LDS; the others clear the target meanwhile.
+template <class T, int E>
 __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(TokenSource src, int npass, int bits, uint32_t* __restrict__ keys, uint32_t* __restrict__ pos,
                                                                   ZeroRows<T> z) {
     if (blockIdx.x > 0) {
         zero_rows(z, blockIdx.x - 1, gridDim.x - 1, kSortThreads);
         return;
     }
-    constexpr int E = kSmallSort / kSortThreads;
-    __shared__ uint32_t lk[kSmallSort];
-    __shared__ uint16_t lp[kSmallSort];
-    __shared__ uint32_t cnt[kSortWaves][kMaxDigits];
+    __shared__ uint32_t lk[kSortThreads * E];
+    __shared__ uint16_t lp[kSortThreads * E];
+    __shared__ uint32_t cnt[kCounters];
     __shared__ uint32_t wave_sum[kSortWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t n = src.n, base = wave * 64 * E + lane;
@@ -190,28 +212,28 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(TokenSource sr
     const uint32_t digits = 1u << bits;
     for (int pass = 0; pass < npass; pass++) {
         const int sh = pass * bits;
-        for (uint32_t d = threadIdx.x; d < kSortWaves * digits; d += kSortThreads) cnt[d >> bits][d & (digits - 1)] = 0;
+        for (uint32_t d = threadIdx.x; d < digits * (kSortWaves + 1); d += kSortThreads) cnt[d] = 0;
         __syncthreads();
         uint32_t digit[E], rank[E];
 #pragma unroll
         for (int e = 0; e < E; e++) digit[e] = (k[e] >> sh) & (digits - 1);
-        wave_ranks<E>(digit, live, bits, cnt[wave], rank);
+        wave_ranks<E>(digit, live, bits, cnt, rank);
         __syncthreads();
-        uint32_t total = 0;
-        if (threadIdx.x < digits)
-            for (int w = 0; w < kSortWaves; w++) {
-                const uint32_t c = cnt[w][threadIdx.x];
-                cnt[w][threadIdx.x] = total;
-                total += c;
-            }
-        const uint32_t start = digit_scan(threadIdx.x < digits ? total : 0u, wave_sum);
-        if (threadIdx.x < digits)
-            for (int w = 0; w < kSortWaves; w++) cnt[w][threadIdx.x] += start;
-        __syncthreads();
+        scan_counters(cnt, bits, wave_sum);
+        if (pass == npass - 1) {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (live[e]) {
+                    const uint32_t to = cnt[counter(digit[e], wave)] + rank[e];
+                    keys[to] = k[e];
+                    pos[to] = p[e];
+                }
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < E; e++)
             if (live[e]) {
-                const uint32_t to = cnt[wave][digit[e]] + rank[e];
+                const uint32_t to = cnt[counter(digit[e], wave)] + rank[e];
                 lk[to] = k[e];
                 lp[to] = (uint16_t)p[e];
             }
@@ -223,12 +245,6 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(TokenSource sr
                 p[e] = lp[base + 64 * e];
             }
     }
-#pragma unroll
-    for (int e = 0; e < E; e++)
-        if (live[e]) {
-            keys[base + 64 * e] = k[e];
-            pos[base + 64 * e] = p[e];
-        }
 }
 
 // One pass through memory, first half: how many tokens of each chunk have each digit -> counts[digit][chunk].
@@ -250,7 +266,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(TokenSource sr
         atomicAdd(&hist[(k >> shift) & (digits - 1)], 1u);
     }
     __syncthreads();
-    if (threadIdx.x < digits) counts[(size_t)threadIdx.x * nchunks + blockIdx.x] = hist[threadIdx.x];
+    if (threadIdx.x < digits) counts[(size_t)blockIdx.x * digits + threadIdx.x] = hist[threadIdx.x];
 }
 
 // Second half: every chunk's tokens go to their places.  A workgroup finds where its share of each digit starts by adding up the
@@ -264,53 +280,57 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(TokenSource sr
         return;
     }
     constexpr int E = kSortTile / kSortThreads;
-    __shared__ uint32_t cnt[kSortWaves][kMaxDigits];
-    __shared__ uint32_t start[kMaxDigits];
+    __shared__ uint32_t cnt[kCounters];
+    __shared__ uint32_t start[kMaxDigits];   // where the chunk's next key of each digit goes
     __shared__ uint32_t wave_sum[kSortWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t digits = 1u << bits;
-    uint32_t total = 0, before = 0;
-    if (threadIdx.x < digits)
-        for (uint32_t c = 0; c < nchunks; c++) {
-            const uint32_t v = counts[(size_t)threadIdx.x * nchunks + c];
-            before += c < blockIdx.x ? v : 0u;
-            total += v;
-        }
-    const uint32_t first = digit_scan(total, wave_sum);
-    if (threadIdx.x < digits) start[threadIdx.x] = first + before;
     const uint32_t i0 = blockIdx.x * chunk, i1 = src.n - i0 < chunk ? src.n : i0 + chunk;
-    for (uint32_t t0 = i0; t0 < i1; t0 += kSortTile) {
-        for (uint32_t d = threadIdx.x; d < kSortWaves * digits; d += kSortThreads) cnt[d >> bits][d & (digits - 1)] = 0;
-        uint32_t k[E], p[E], digit[E], rank[E];
-        bool live[E];
+    uint32_t k[E], p[E];
+    auto load = [&](uint32_t t0) {
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const uint32_t i = t0 + wave * 64 * E + 64 * e + lane;
-            live[e] = i < i1;
-            k[e] = !live[e] ? 0u : keys ? keys[i] : token_key(src, i);
-            p[e] = !live[e] ? 0u : keys ? pos[i] : i;
+            k[e] = i >= i1 ? 0u : keys ? keys[i] : token_key(src, i);
+            p[e] = i >= i1 ? 0u : keys ? pos[i] : i;
+        }
+    };
+    load(i0);                                // in flight while the counts are added up
+    uint32_t total = 0, before = 0;
+    if (threadIdx.x < digits)
+#pragma unroll 8
+        for (uint32_t c = 0; c < nchunks; c++) {
+            const uint32_t v = counts[(size_t)c * digits + threadIdx.x];
+            before += c < blockIdx.x ? v : 0u;
+            total += v;
+        }
+    const uint32_t first = block_scan(total, wave_sum);
+    if (threadIdx.x < digits) start[threadIdx.x] = first + before;
+    for (uint32_t t0 = i0; t0 < i1; t0 += kSortTile) {
+        for (uint32_t d = threadIdx.x; d < digits * (kSortWaves + 1); d += kSortThreads) cnt[d] = 0;
+        if (t0 != i0) load(t0);
+        uint32_t digit[E], rank[E];
+        bool live[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            live[e] = t0 + wave * 64 * E + 64 * e + lane < i1;
             digit[e] = (k[e] >> shift) & (digits - 1);
         }
         __syncthreads();
-        wave_ranks<E>(digit, live, bits, cnt[wave], rank);
+        wave_ranks<E>(digit, live, bits, cnt, rank);
         __syncthreads();
-        if (threadIdx.x < digits) {
-            uint32_t run = start[threadIdx.x];
-            for (int w = 0; w < kSortWaves; w++) {
-                const uint32_t c = cnt[w][threadIdx.x];
-                cnt[w][threadIdx.x] = run;
-                run += c;
-            }
-            start[threadIdx.x] = run;
-        }
-        __syncthreads();
+        scan_counters(cnt, bits, wave_sum);
 #pragma unroll
         for (int e = 0; e < E; e++)
             if (live[e]) {
-                const uint32_t to = cnt[wave][digit[e]] + rank[e];
+                const uint32_t to = start[digit[e]] + cnt[counter(digit[e], wave)] - cnt[counter(digit[e], 0)] + rank[e];
                 keys_out[to] = k[e];
                 pos_out[to] = p[e];
             }
+        __syncthreads();
+        // (the last wavefront's start of a digit, and what it has of it itself, are where the next tile goes on)
+        if (t0 + kSortTile < i1 && threadIdx.x < digits)
+            start[threadIdx.x] += (threadIdx.x + 1 < digits ? cnt[counter(threadIdx.x + 1, 0)] : kSortTile) - cnt[counter(threadIdx.x, 0)];
         __syncthreads();
     }
 }
@@ -353,8 +373,17 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(GradTarget<T> tg,
         for (int e = 0; e < live; e++) partial[((size_t)piece * 2 + which) * pitch + c + e] = acc[e];
     };
     auto to_row = [&]() {
-        if (cur != vocab)
+        if (cur == vocab) return;
+        if (VEC && live == N && tg.d_stride == 1) {
+            V* p = (V*)(tg.t + (int64_t)cur * tg.row_stride + c);
+            V v = 0;
+            if (tg.accumulate) v = *p;
+#pragma unroll
+            for (int e = 0; e < N; e++) v[e] = (T)((double)v[e] + acc[e] * tg.scale);
+            *p = v;
+        } else {
             for (int e = 0; e < live; e++) put(tg, cur, c + e, acc[e]);
+        }
     };
     for (uint32_t i = i0; i < i1; i += U) {
         uint32_t k[U];
@@ -395,17 +424,18 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(GradTarget<T> tg,
     else to_row();
 }
 
-// Runs that cross pieces.  The workgroups of the piece in which such a run begins add its partials: 128 columns each, the pieces dealt
-// to eight wavefronts, whose sums are added in order.
-constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64, kJoinCols = 128;
+// Runs that cross pieces.  The workgroups of the piece in which such a run begins add its partials: 256 columns each, the pieces dealt
+// to four wavefronts, whose sums are added in order.
+constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kJoinCols = 256;
 template <class T>
 __global__ __launch_bounds__(kJoinThreads) void embedding_join_kernel(GradTarget<T> tg, const uint32_t* __restrict__ keys, uint32_t n, uint32_t vocab, uint32_t R,
                                                                       uint32_t pieces, int64_t pitch, const double* __restrict__ partial) {
+    typedef double D2 __attribute__((ext_vector_type(2)));
     const uint32_t piece = blockIdx.x, i0 = piece * R, i1 = n - i0 < R ? n : i0 + R;
     if (i1 >= n) return;
-    const uint32_t key = keys[i1 - 1];
-    if (key == vocab || keys[i1] != key) return;                              // no run goes on behind this piece
-    if (keys[i0] == key && i0 > 0 && keys[i0 - 1] == key) return;             // one does, but it began earlier
+    const uint32_t key = keys[i1 - 1], after = keys[i1], head = keys[i0], before = i0 > 0 ? keys[i0 - 1] : vocab;
+    if (key == vocab || after != key) return;                                 // no run goes on behind this piece
+    if (head == key && before == key) return;                                 // one does, but it began earlier
     __shared__ double sums[kJoinWaves][kJoinCols];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t more = 0;                                                        // pieces that continue the run
@@ -418,26 +448,24 @@ __global__ __launch_bounds__(kJoinThreads) void embedding_join_kernel(GradTarget
         }
         more += 64;
     }
-    const int64_t c = (int64_t)blockIdx.y * kJoinCols + 2 * lane;             // the pitch is even: a lane's two columns exist in the partials
-    const bool in = c < tg.width;
-    double a0 = 0, a1 = 0;
-    if (in)
+    // a lane takes columns 2 l, 2 l + 1 and those 128 further on; the pitch is even, so a pair that begins in the row exists in the partials
+    const int64_t c0 = (int64_t)blockIdx.y * kJoinCols + 2 * lane, c1 = c0 + kJoinCols / 2;
+    const int64_t r0 = c0 < tg.width ? c0 : 0, r1 = c1 < tg.width ? c1 : 0;
+    D2 a0 = 0, a1 = 0;
 #pragma unroll 8
-        for (uint32_t q = wave; q <= more; q += kJoinWaves) {
-            const double* p = partial + ((size_t)(piece + q) * 2 + (q == 0 ? 1 : 0)) * pitch + c;
-            a0 += p[0];
-            a1 += c + 1 < tg.width ? p[1] : 0.0;
-        }
-    sums[wave][2 * lane] = a0;
-    sums[wave][2 * lane + 1] = a1;
+    for (uint32_t q = wave; q <= more; q += kJoinWaves) {
+        const double* p = partial + ((size_t)(piece + q) * 2 + (q == 0 ? 1 : 0)) * pitch;
+        a0 += *(const D2*)(p + r0);
+        a1 += *(const D2*)(p + r1);
+    }
+    *(D2*)&sums[wave][2 * lane] = a0;
+    *(D2*)&sums[wave][kJoinCols / 2 + 2 * lane] = a1;
     __syncthreads();
-    if (threadIdx.x < kJoinCols) {
-        const int64_t cc = (int64_t)blockIdx.y * kJoinCols + threadIdx.x;
-        if (cc < tg.width) {
-            double v = 0;
-            for (int w = 0; w < kJoinWaves; w++) v += sums[w][threadIdx.x];
-            put(tg, key, cc, v);
-        }
+    const int64_t c = (int64_t)blockIdx.y * kJoinCols + threadIdx.x;
+    if (c < tg.width) {
+        double v = 0;
+        for (int w = 0; w < kJoinWaves; w++) v += sums[w][threadIdx.x];
+        put(tg, key, c, v);
     }
 }
 
@@ -455,8 +483,9 @@ GradPlan grad_plan(uint32_t n, int64_t vocab, int64_t width) {
     while (((int64_t)1 << kb) <= vocab) kb++;   // keys are 0 .. vocab
     p.npass = (kb + kMaxDigitBits - 1) / kMaxDigitBits;
     p.bits = (kb + p.npass - 1) / p.npass;
+    if (p.bits < kMinDigitBits) p.bits = kMinDigitBits;
     // pieces of 8 to 32 tokens: enough of them to fill the chip, and long enough that partials stay rare
-    uint32_t R = (n + 2047) / 2048;
+    uint32_t R = (n + 1023) / 1024;
     R = (R + 7) / 8 * 8;
     p.R = R < 8 ? 8 : R > 32 ? 32 : R;
     p.pieces = cdiv(n, p.R);
@@ -488,7 +517,7 @@ int32_t embedding_grad(const DnhTensor* dt, const DnhTensor* tokens, const DnhTe
     const unsigned fill_wgs = accumulate ? 0 : (unsigned)(2 * device_cus());
     if (n == 0) {
         if (accumulate) return DNH_OK;
-        hipLaunchKernelGGL((sort_small_kernel<T>), dim3(1 + fill_wgs), dim3(kSortThreads), 0, s, src, 0, 1, nullptr, nullptr, z);
+        hipLaunchKernelGGL((sort_small_kernel<T, 1>), dim3(1 + fill_wgs), dim3(kSortThreads), 0, s, src, 0, kMinDigitBits, nullptr, nullptr, z);
         DNH_LAUNCH_CHECK();
         return DNH_OK;
     }
@@ -500,26 +529,30 @@ int32_t embedding_grad(const DnhTensor* dt, const DnhTensor* tokens, const DnhTe
     double* partial = (double*)(rest + p.counts_bytes);
     int cur = 0;
     if (n <= kSmallSort) {
-        hipLaunchKernelGGL((sort_small_kernel<T>), dim3(1 + fill_wgs), dim3(kSortThreads), 0, s, src, p.npass, p.bits, list[0][0], list[0][1], z);
+#define SORT(E) hipLaunchKernelGGL((sort_small_kernel<T, E>), dim3(1 + fill_wgs), dim3(kSortThreads), 0, s, src, p.npass, p.bits, list[0][0], list[0][1], z)
+        if (n <= kSortThreads) SORT(1);
+        else if (n <= 4 * kSortThreads) SORT(4);
+        else SORT(8);
+#undef SORT
         DNH_LAUNCH_CHECK();
     } else {
-        // each of the 2 npass launches clears its share of the target beside the sort
-        const int launches = 2 * p.npass;
+        // every launch of the sort clears a share of the target beside it: counting takes about half the time of placing
+        const int parts = 3 * p.npass;
         int done = 0;
-        auto share = [&]() {
+        auto share = [&](int some) {
             ZeroRows<T> part = z;
-            part.row0 = z.row1 * done / launches;
-            part.row1 = z.row1 * (done + 1) / launches;
-            done++;
+            part.row0 = z.row1 * done / parts;
+            done += some;
+            part.row1 = z.row1 * done / parts;
             return part;
         };
         for (int pass = 0; pass < p.npass; pass++) {
             const uint32_t* ki = pass ? list[cur][0] : nullptr;
             const uint32_t* pi = pass ? list[cur][1] : nullptr;
-            hipLaunchKernelGGL((sort_count_kernel<T>), dim3(p.nchunks + fill_wgs), dim3(kSortThreads), 0, s, src, ki, pass * p.bits, p.bits, p.chunk, p.nchunks, counts, share());
+            hipLaunchKernelGGL((sort_count_kernel<T>), dim3(p.nchunks + fill_wgs), dim3(kSortThreads), 0, s, src, ki, pass * p.bits, p.bits, p.chunk, p.nchunks, counts, share(1));
             DNH_LAUNCH_CHECK();
             hipLaunchKernelGGL((sort_place_kernel<T>), dim3(p.nchunks + fill_wgs), dim3(kSortThreads), 0, s, src, ki, pi, pass * p.bits, p.bits, p.chunk, p.nchunks,
-                               (const uint32_t*)counts, list[cur ^ 1][0], list[cur ^ 1][1], share());
+                               (const uint32_t*)counts, list[cur ^ 1][0], list[cur ^ 1][1], share(2));
             DNH_LAUNCH_CHECK();
             cur ^= 1;
         }
