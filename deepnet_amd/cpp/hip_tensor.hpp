@@ -224,6 +224,20 @@ template <class T> class Tensor;
 template <class T>
 inline DnhTensor desc(const Tensor<T>& t);
 
+// Device memory for the intermediates of a language-model operator; none: the stream's workspace.
+struct Scratch {
+    void* ptr = nullptr;
+    size_t bytes = 0;
+};
+// Descriptor of a tensor that may be left out (p stays nullptr).
+struct OptDesc {
+    DnhTensor d{};
+    const DnhTensor* p = nullptr;
+    template <class X> explicit OptDesc(const Tensor<X>* t) {
+        if (t) { d = desc(*t); p = &d; }
+    }
+};
+
 // ---- ITensorBackend<'T> (TensorBackend.fs:64-146) ----------------------------------------------------------------------------------
 template <class T>
 struct TensorHipBackend {
@@ -332,6 +346,38 @@ struct TensorHipBackend {
     static void MatVecDot(const Tensor<T>& t, const Tensor<T>& a, const Tensor<T>& b) { dot(t, a, b); }
     static void MatMatDot(const Tensor<T>& t, const Tensor<T>& a, const Tensor<T>& b) { dot(t, a, b); }
     static void BatchedMatMatDot(const Tensor<T>& t, const Tensor<T>& a, const Tensor<T>& b) { dot(t, a, b); }
+    // Operators of language models (no counterpart in ITensorBackend; include/tensor_hip.h states their contracts).  nullptr leaves a tensor
+    // or the scale out; Scratch: device memory for the intermediates of a call that is captured into a graph.
+    static void Embedding(const Tensor<T>& trgt, const Tensor<T>& table, const Tensor<int64_t>& tokens, const T* scale = nullptr) {
+        auto t = desc(trgt); auto w = desc(table); auto k = desc(tokens);
+        check(dnh_embedding(&t, &w, &k, scale, Cfg::Stream())); checkIndexError();
+    }
+    static void EmbeddingGrad(const Tensor<T>& trgt, const Tensor<int64_t>& tokens, const Tensor<T>& dOut, const T* scale = nullptr, bool accumulate = false, Scratch s = {}) {
+        auto t = desc(trgt); auto k = desc(tokens); auto g = desc(dOut);
+        check(dnh_embedding_grad(&t, &k, &g, scale, accumulate ? 1 : 0, s.ptr, s.bytes, Cfg::Stream())); checkIndexError();
+    }
+    static void TokenLogProbs(const Tensor<T>* logProbs, const Tensor<T>* lse, const Tensor<T>* entropy, const Tensor<T>* topLogProbs, const Tensor<int64_t>* topTokens,
+                              const Tensor<T>& logits, const Tensor<int64_t>* tokens, Scratch s = {}) {
+        OptDesc a(logProbs), b(lse), c(entropy), d(topLogProbs), e(topTokens), k(tokens); auto x = desc(logits);
+        check(dnh_token_log_probs(a.p, b.p, c.p, d.p, e.p, &x, k.p, s.ptr, s.bytes, Cfg::Stream()));
+        if (tokens) checkIndexError();
+    }
+    static void TokenLogProbsGrad(const Tensor<T>& trgt, const Tensor<T>& logits, const Tensor<int64_t>& tokens, const Tensor<T>& lse, const Tensor<T>* entropy,
+                                  const Tensor<T>& dLogProbs, const Tensor<T>* dEntropy) {
+        auto t = desc(trgt); auto x = desc(logits); auto k = desc(tokens); auto l = desc(lse); auto g = desc(dLogProbs); OptDesc e(entropy), h(dEntropy);
+        check(dnh_token_log_probs_grad(&t, &x, &k, &l, e.p, &g, h.p, Cfg::Stream())); checkIndexError();
+    }
+    static void CrossAttention(const Tensor<T>& trgt, const Tensor<T>* lse, const Tensor<T>& q, const Tensor<T>& k, const Tensor<T>& v, const Tensor<bool>* mask = nullptr,
+                               const T* scale = nullptr, Scratch s = {}) {
+        auto t = desc(trgt); auto a = desc(q); auto b = desc(k); auto c = desc(v); OptDesc l(lse), m(mask);
+        check(dnh_cross_attention(&t, l.p, &a, &b, &c, m.p, scale, s.ptr, s.bytes, Cfg::Stream()));
+    }
+    static void CrossAttentionGrad(const Tensor<T>* dQ, const Tensor<T>* dK, const Tensor<T>* dV, const Tensor<T>& dOut, const Tensor<T>& q, const Tensor<T>& k,
+                                   const Tensor<T>& v, const Tensor<T>& out, const Tensor<T>& lse, const Tensor<bool>* mask = nullptr, const T* scale = nullptr, Scratch s = {}) {
+        OptDesc tq(dQ), tk(dK), tv(dV), m(mask); auto g = desc(dOut); auto a = desc(q); auto b = desc(k); auto c = desc(v); auto o = desc(out); auto l = desc(lse);
+        check(dnh_cross_attention_grad(tq.p, tk.p, tv.p, &g, &a, &b, &c, &o, &l, m.p, scale, s.ptr, s.bytes, Cfg::Stream()));
+    }
+
     static void BatchedInvert(const Tensor<T>& trgt, const Tensor<T>& src) { auto t = desc(trgt); auto s = desc(src); check(dnh_batched_invert(&t, &s, Cfg::Stream())); }
     // trgtU / trgtV both null: singular values only (the reference's `trgtUV: (U, V) option`)
     static void BatchedSVD(const Tensor<T>& trgtS, const Tensor<T>* trgtU, const Tensor<T>* trgtV, const Tensor<T>& src) {
@@ -344,6 +390,8 @@ struct TensorHipBackend {
         check(dnh_symmetric_eig(part == MatrixPart::Upper ? 0 : 1, &w, &v, &a, Cfg::Stream()));
     }
 };
+
+template <class T> struct LogProbs;   // results of Tensor<T>::tokenLogProbs
 
 // ---- Tensor<'T> frontend (Tensor.fs), the part that drives the backend path -----------------------------------------------------------
 template <class T>
@@ -525,6 +573,57 @@ class Tensor {
         Backend::MaskedSet(Relayout(*view), {&fm}, value.broadcastTo(Shape{mask.countTrue()}));
     }
 
+    // operators of language models (no counterpart in Tensor.fs); the targets' shapes are those include/tensor_hip.h states
+    static Tensor embedding(const Tensor& table, const Tensor<int64_t>& tokens, T scale = T(1)) {
+        if (table.NDims() != 2) throw std::invalid_argument("An embedding table must be a matrix.");
+        Shape shp = tokens.Shape_();
+        shp.push_back(table.Shape_()[1]);
+        Tensor t(shp);
+        Backend::Embedding(t, table, tokens, &scale);
+        return t;
+    }
+    static Tensor embeddingGrad(const Tensor<int64_t>& tokens, const Tensor& dOut, int64_t vocab, T scale = T(1)) {
+        if (dOut.NDims() < 1) throw std::invalid_argument("dOut needs a last axis of the table's row length.");
+        Tensor t(Shape{vocab, dOut.Shape_().back()});
+        Backend::EmbeddingGrad(t, tokens, dOut, &scale);
+        return t;
+    }
+    static LogProbs<T> tokenLogProbs(const Tensor& logits, const Tensor<int64_t>& tokens, int64_t top = 0) {
+        if (logits.NDims() < 1) throw std::invalid_argument("Logits need a last axis of alternatives.");
+        Shape row = logits.Shape_(), best = row;
+        row.pop_back();
+        best.back() = top;
+        LogProbs<T> r{Tensor(row), Tensor(row), Tensor(row), Tensor(best), Tensor<int64_t>(best)};
+        Backend::TokenLogProbs(&r.logProbs, &r.lse, &r.entropy, top ? &r.topLogProbs : nullptr, top ? &r.topTokens : nullptr, logits, &tokens);
+        return r;
+    }
+    static Tensor tokenLogProbsGrad(const Tensor& logits, const Tensor<int64_t>& tokens, const Tensor& lse, const Tensor& dLogProbs, const Tensor* entropy = nullptr,
+                                    const Tensor* dEntropy = nullptr) {
+        Tensor t(logits.Shape_());
+        Backend::TokenLogProbsGrad(t, logits, tokens, lse, entropy, dLogProbs, dEntropy);
+        return t;
+    }
+    struct Attention {
+        Tensor out, lse;
+    };
+    static Attention crossAttention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor<bool>* mask = nullptr, const T* scale = nullptr) {
+        if (q.NDims() != 4 || v.NDims() != 4) throw std::invalid_argument("q and v must have the axes [batch; head; position; width].");
+        Shape shp = q.Shape_(), row(shp.begin(), shp.begin() + 3);
+        shp[3] = v.Shape_()[3];
+        Attention r{Tensor(shp), Tensor(row)};
+        Backend::CrossAttention(r.out, &r.lse, q, k, v, mask, scale);
+        return r;
+    }
+    struct AttentionGrads {
+        Tensor dQ, dK, dV;
+    };
+    static AttentionGrads crossAttentionGrad(const Tensor& dOut, const Tensor& q, const Tensor& k, const Tensor& v, const Attention& a, const Tensor<bool>* mask = nullptr,
+                                             const T* scale = nullptr) {
+        AttentionGrads r{Tensor(q.Shape_()), Tensor(k.Shape_()), Tensor(v.Shape_())};
+        Backend::CrossAttentionGrad(&r.dQ, &r.dK, &r.dV, dOut, q, k, v, a.out, a.lse, mask, scale);
+        return r;
+    }
+
     // (batched) matrix inverse (Tensor.fs:2807-2839)
     void FillInvert(const Tensor& a) const {
         if (a.NDims() < 2) throw std::invalid_argument("Need at least a matrix to invert.");
@@ -588,6 +687,11 @@ class Tensor {
   private:
     TensorLayout layout_;
     std::shared_ptr<TensorHipStorage<T>> storage_;
+};
+
+template <class T> struct LogProbs {
+    Tensor<T> logProbs, lse, entropy, topLogProbs;
+    Tensor<int64_t> topTokens;
 };
 
 template <class T>

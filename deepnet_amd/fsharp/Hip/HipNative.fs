@@ -105,6 +105,18 @@ module internal Native =
     [<DllImport(Lib, CallingConvention=CallingConvention.Cdecl, EntryPoint="dnh_batched_svd")>] extern int dnh_batched_svd_values (DnhTensor& s, nativeint u, nativeint v, DnhTensor& src, nativeint stream)
     [<DllImport(Lib, CallingConvention=CallingConvention.Cdecl)>] extern int dnh_symmetric_eig (int part, DnhTensor& eigVals, DnhTensor& eigVecs, DnhTensor& src, nativeint stream)
 
+    // Operators of language models: descriptors cross by address, IntPtr.Zero where a tensor is left out (HipModel builds them), as do the
+    // scale and the scratch memory.
+    [<DllImport(Lib, CallingConvention=CallingConvention.Cdecl, EntryPoint="dnh_embedding")>] extern int embedding (nativeint t, nativeint table, nativeint tokens, nativeint scale, nativeint stream)
+    [<DllImport(Lib, CallingConvention=CallingConvention.Cdecl, EntryPoint="dnh_embedding_grad")>] extern int embedding_grad (nativeint dTable, nativeint tokens, nativeint dOut, nativeint scale, int accumulate, nativeint scratch, unativeint scratchBytes, nativeint stream)
+    [<DllImport(Lib, CallingConvention=CallingConvention.Cdecl, EntryPoint="dnh_token_log_probs")>] extern int token_log_probs (nativeint logProbs, nativeint lse, nativeint entropy, nativeint topLogProbs, nativeint topTokens, nativeint logits, nativeint tokens, nativeint scratch, unativeint scratchBytes, nativeint stream)
+    [<DllImport(Lib, CallingConvention=CallingConvention.Cdecl, EntryPoint="dnh_token_log_probs_grad")>] extern int token_log_probs_grad (nativeint dLogits, nativeint logits, nativeint tokens, nativeint lse, nativeint entropy, nativeint dLogProbs, nativeint dEntropy, nativeint stream)
+    [<DllImport(Lib, CallingConvention=CallingConvention.Cdecl, EntryPoint="dnh_cross_attention")>] extern int cross_attention (nativeint out, nativeint lse, nativeint q, nativeint k, nativeint v, nativeint mask, nativeint scale, nativeint scratch, unativeint scratchBytes, nativeint stream)
+    [<DllImport(Lib, CallingConvention=CallingConvention.Cdecl, EntryPoint="dnh_cross_attention_grad")>] extern int cross_attention_grad (nativeint dQ, nativeint dK, nativeint dV, nativeint dOut, nativeint q, nativeint k, nativeint v, nativeint out, nativeint lse, nativeint mask, nativeint scale, nativeint scratch, unativeint scratchBytes, nativeint stream)
+    [<DllImport(Lib, CallingConvention=CallingConvention.Cdecl)>] extern int dnh_embedding_grad_scratch_bytes (int64 tokens, int64 vocab, int64 width, unativeint& bytes)
+    [<DllImport(Lib, CallingConvention=CallingConvention.Cdecl)>] extern int dnh_token_log_probs_scratch_bytes (int dtype, int64 rows, int64 vocab, int64 top, unativeint& bytes)
+    [<DllImport(Lib, CallingConvention=CallingConvention.Cdecl)>] extern int dnh_cross_attention_scratch_bytes (int dtype, int64 batch, int64 heads, int64 kvHeads, int64 queries, int64 keys, int64 width, unativeint& bytes)
+
     /// Maps a status to the exception type the reference's backends raise for the same condition.
     let check (status: int) =
         if status <> 0 then
