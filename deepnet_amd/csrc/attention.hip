@@ -15,6 +15,18 @@ constexpr int64_t kMaxHeadWidth = 128;
 
 Strides4 strides4(const DnhTensor* t) { return Strides4{t->stride[0], t->stride[1], t->stride[2], t->ndims > 3 ? t->stride[3] : 0}; }
 
+// 32-bit counts inside the kernels (extents, rows of a key head, heads), and grids of fewer than 2^32 threads: at most 2^23 tiles of 64 rows,
+// as many of 64 keys, and 2^28 rows for the kernels that give each 16 lanes or more
+int32_t check_extents(int64_t batch, int64_t heads, int64_t kv_heads, int64_t queries, int64_t keys, const char* what) {
+    const int64_t lim = 0x7FFFFFFF - 16384;
+    if (batch > lim || heads > lim || kv_heads > lim || queries > lim || keys > lim) return fail(DNH_ERR_NOT_SUPPORTED, "%s: an extent of 2^31 or more", what);
+    if (kv_heads == 0) return DNH_OK;
+    const int64_t rows = heads / kv_heads * queries, n = batch * kv_heads;
+    if (n > (1 << 23) || rows > lim || n * (rows / 32 + 1) >= (1 << 23) || n * (keys / 64 + 1) >= (1 << 23))
+        return fail(DNH_ERR_NOT_SUPPORTED, "%s: more than 2^23 tiles of rows or keys", what);
+    return DNH_OK;
+}
+
 // The operands both directions share: q [B; Hq; Lq; Dk], k [B; Hk; Lk; Dk], v [B; Hk; Lk; Dv], mask [B; Lk] or NULL
 int32_t check_operands(const DnhTensor* q, const DnhTensor* k, const DnhTensor* v, const DnhTensor* mask, const char* what) {
     const DnhTensor* ts[] = {q, k, v};
@@ -36,15 +48,7 @@ int32_t check_operands(const DnhTensor* q, const DnhTensor* k, const DnhTensor* 
         if (mask->dtype != DNH_BOOL || mask->ndims != 2 || mask->shape[0] != k->shape[0] || mask->shape[1] != k->shape[2])
             return fail(DNH_ERR_INVALID_ARG, "%s: the mask must be a bool tensor [batch; key position]", what);
     }
-    // 32-bit counts inside the kernels: rows of a key head, positions, workgroups
-    const int64_t lim = 0x7FFFFFFF - 4096;
-    if (q->shape[0] > lim || q->shape[1] > lim || q->shape[2] > lim || k->shape[2] > lim) return fail(DNH_ERR_NOT_SUPPORTED, "%s: an extent of 2^31 or more", what);
-    if (k->shape[1]) {
-        const int64_t rows = q->shape[1] / k->shape[1] * q->shape[2], heads = q->shape[0] * k->shape[1];
-        if (rows > lim || heads > lim || heads * (rows / 16 + 1) > (1 << 22) || heads * (k->shape[2] / 16 + 1) > (1 << 22))
-            return fail(DNH_ERR_NOT_SUPPORTED, "%s: more than 2^22 tiles of rows or keys", what);
-    }
-    return DNH_OK;
+    return check_extents(q->shape[0], q->shape[1], k->shape[1], q->shape[2], k->shape[2], what);
 }
 
 int32_t check_like(const DnhTensor* t, const DnhTensor* q, int64_t heads, int64_t len, int64_t width, const char* what, const char* name, bool target) {
@@ -140,6 +144,7 @@ extern "C" int32_t dnh_cross_attention_scratch_bytes(int32_t dtype, int64_t batc
                                                      size_t* bytes) {
     if (!bytes || !dtype_is_fp(dtype) || batch < 0 || kv_heads < 1 || heads < 0 || heads % kv_heads != 0 || queries < 0 || keys < 0 || width < 1 || width > kMaxHeadWidth)
         return fail(DNH_ERR_INVALID_ARG, "dnh_cross_attention_scratch_bytes: bad argument");
+    DNH_TRY(check_extents(batch, heads, kv_heads, queries, keys, "dnh_cross_attention_scratch_bytes"));
     const int64_t n = batch * kv_heads, rows = heads / kv_heads * queries;
     *bytes = 0;
     if (n == 0 || rows == 0) return DNH_OK;

@@ -518,7 +518,7 @@ __global__ __launch_bounds__(64) void attention_few_kernel(AttArgs<typename A::T
             if (on == 0) continue;
             const int key0 = t * kAttTile + part * KEYS;
             V ka[NS][NT], va[NS][A::R][NG];
-            auto load = [&](const T* base, int d, int D, int64_t sd) {   // (what lies beyond Dk meets zeros of the query, beyond Dv is not stored)
+            auto load = [&](const T* base, int d, int D, int64_t sd) {   // (what lies beyond Dk is cleared below, what lies beyond Dv not stored)
                 if constexpr (WHOLE) return *(const V*)(base + (d < D ? d : 0));
                 else return att_load<T>(base, d, D, sd, p.vec);
             };
@@ -538,6 +538,13 @@ __global__ __launch_bounds__(64) void attention_few_kernel(AttArgs<typename A::T
 #pragma unroll
                     for (int g = 0; g < NG; g++) va[u][r][g] = load(vr, (16 * g + c) * N, p.Dv, p.sv.d);
                 }
+            if (WHOLE && p.Dk < DP) {   // (an infinity among the keys must not meet the query's zeros)
+#pragma unroll
+                for (int u = 0; u < NS; u++)
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+                        if (GN * i + h * N >= p.Dk) ka[u][i] = 0;
+            }
             Acc s[NS];
 #pragma unroll
             for (int u = 0; u < NS; u++) {
@@ -819,6 +826,10 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
         ov = p.part_dv + at_row * p.Dv;
         sk = sv = 1;
     }
+    if (!on) {   // zero, whatever d_out holds: an infinity there has met the key's zero probabilities
+#pragma unroll
+        for (int i = 0; i < ND; i++) dk[i] = dv[i] = 0;
+    }
     Ops::put(ok, sk, p.Dk, dk, T(1), h);
     Ops::put(ov, sv, p.Dv, dv, T(1), h);
 }
@@ -886,12 +897,16 @@ inline double att_walk_us(int64_t width, int products, int64_t tiles) {
 // `n` workgroups of `each` us on `slots` places: what a place has to do on average, and half a walk for the uneven end
 inline double att_span_us(double n, double each, double slots) { return n <= slots ? each : n * each / slots + 0.5 * each; }
 inline double att_join_us(double bytes) { return bytes > 0 ? 5.0 + 2 * bytes / 4.0e6 : 0.0; }
+// Most memory for the parts of a walk that is shared: 256 MB, which the Infinity Cache holds between the two launches.  A walk that would
+// need more has workgroups enough to fill the chip many times over, and its uneven end costs it little.
+constexpr double kAttPartBytes = 256.0 * 1024 * 1024;
 
 struct AttPlan {
     int waves;   // 0: the kernel for few rows
     uint32_t blocks, splits, split_tiles;
     size_t o_bytes, m_bytes, total;
 };
+// The shares depend on the larger width alone, so that the memory they need for Dk = Dv = width is enough for every smaller one.
 template <class T> AttPlan att_plan(int64_t heads, int64_t rows, int64_t Lk, int64_t Dk, int64_t Dv) {
     constexpr int M = MmaOf<T>::Tile::M;
     AttPlan p;
@@ -908,8 +923,9 @@ template <class T> AttPlan att_plan(int64_t heads, int64_t rows, int64_t Lk, int
         double best = 0;
         for (int64_t n = 1; n <= 64 && (n == 1 || 2 * n <= tiles + 1); n++) {
             const int64_t each = (tiles + n - 1) / n;
-            const double us = att_span_us((double)heads * p.blocks * n, att_walk_us(width, 2, each), slots) + att_join_us(n > 1 ? (double)heads * rows * n * Dv * sizeof(T) : 0.0);
-            if (n > 1 && us >= best) continue;
+            const double bytes = n > 1 ? (double)heads * rows * n * width * sizeof(T) : 0.0;
+            const double us = att_span_us((double)heads * p.blocks * n, att_walk_us(width, 2, each), slots) + att_join_us(bytes);
+            if (n > 1 && (us >= best || bytes > kAttPartBytes)) continue;
             best = us;
             p.split_tiles = (uint32_t)(each < 1 ? 1 : each);
             p.splits = cdiv(tiles, p.split_tiles);
@@ -941,9 +957,9 @@ template <class T> AttGradPlan att_grad_plan(int64_t heads, int64_t rows, int64_
             const int64_t eq = (tk + n - 1) / n, ek = (tr + k - 1) / k;
             const double uq = att_walk_us(width, 3, eq), uk = att_walk_us(width, 4, ek), longest = uq > uk ? uq : uk;
             const double even = (qn * n * uq + kn * k * uk) / slots + 0.5 * (uq < uk ? uq : uk);
-            const double bytes = (n > 1 ? (double)heads * rows * Dk * n : 0.0) + (k > 1 ? (double)heads * Lk * (Dk + Dv) * k : 0.0);
-            const double us = (qn * n + kn * k <= slots || even < longest ? longest : even) + att_join_us(bytes * sizeof(T));
-            if ((n > 1 || k > 1) && us >= best) continue;
+            const double bytes = ((n > 1 ? (double)heads * rows * n : 0.0) + (k > 1 ? (double)heads * Lk * 2 * k : 0.0)) * width * sizeof(T);
+            const double us = (qn * n + kn * k <= slots || even < longest ? longest : even) + att_join_us(bytes);
+            if ((n > 1 || k > 1) && (us >= best || bytes > kAttPartBytes)) continue;
             best = us;
             p.split_tiles = (uint32_t)(eq < 1 ? 1 : eq);
             p.splits = cdiv(tk, p.split_tiles);

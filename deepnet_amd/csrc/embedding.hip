@@ -69,6 +69,7 @@ int32_t launch_embedding(const DnhTensor* t, const DnhTensor* table, const DnhTe
     // four rows per thread once the rows alone fill the chip; one where that would leave compute units idle
     const bool deep = (int64_t)cdiv(n, per * 4) * gy >= 2 * device_cus();
     const dim3 grid(cdiv(n, per * (deep ? 4 : 1)), gy);
+    if (grid.x >= 1u << 24) return fail(DNH_ERR_NOT_SUPPORTED, "dnh_embedding: %u rows of %lld elements are more than one call can address", n, (long long)width);
 #define ARGS (T*)elem_ptr(t), (const T*)elem_ptr(table), (const int64_t*)elem_ptr(tokens), rp, n, t->stride[nd], table->stride[0], table->stride[1], \
              table->shape[0], width, scale, txl, err
     if (deep) hipLaunchKernelGGL((embedding_kernel<T, VEC, 4>), grid, dim3(kBlock), 0, s, ARGS);

@@ -751,7 +751,7 @@ class Tensor:
 
     def FillEmbeddingGrad(self, tokens: "Tensor", dOut: "Tensor", scale=None, accumulate=False, scratch=None):
         """self[v, :] = scale * sum of dOut[i, :] over the i with tokens[i] = v; accumulate=True adds that to self."""
-        _same_storage([self, tokens, dOut])
+        _same_storage([self, tokens, dOut, scratch])
         self._model_op("EmbeddingGrad")(self, tokens, dOut, scale, accumulate, scratch)
 
     @staticmethod
@@ -766,7 +766,7 @@ class Tensor:
     def FillTokenLogProbs(logits: "Tensor", tokens=None, logProbs=None, lse=None, entropy=None, topLogProbs=None, topTokens=None, scratch=None):
         """Fills the given targets from logits [i_1 .. i_n; V]: log probabilities of tokens [i], lse and entropy [i] of each row, the
         largest log probabilities and their tokens [i; K]."""
-        _same_storage([logits, tokens, logProbs, lse, entropy, topLogProbs, topTokens])
+        _same_storage([logits, tokens, logProbs, lse, entropy, topLogProbs, topTokens, scratch])
         logits._model_op("TokenLogProbs")(logProbs, lse, entropy, topLogProbs, topTokens, logits, tokens, scratch)
 
     @staticmethod
@@ -794,7 +794,7 @@ class Tensor:
     def FillCrossAttention(self, q, k, v, mask=None, scale=None, lse=None, scratch=None):
         """self = softmax(scale q k^T) v over the keys for which mask [batch; position] is true, lse the logarithm of each row's sum of
         exponentials.  q [batch; head; position; width]; k and v may have fewer heads, each shared by neighbouring query heads."""
-        _same_storage([self, q, k, v, mask, lse])
+        _same_storage([self, q, k, v, mask, lse, scratch])
         self._model_op("CrossAttention")(self, lse, q, k, v, mask, scale, scratch)
 
     @staticmethod
@@ -810,7 +810,7 @@ class Tensor:
     @staticmethod
     def FillCrossAttentionGrad(dQ, dK, dV, dOut, q, k, v, out, lse, mask=None, scale=None, scratch=None):
         """Gradients of sum(dOut out) into dQ, dK and dV; dQ, or dK and dV, may be None."""
-        _same_storage([dQ, dK, dV, dOut, q, k, v, out, lse, mask])
+        _same_storage([dQ, dK, dV, dOut, q, k, v, out, lse, mask, scratch])
         q._model_op("CrossAttentionGrad")(dQ, dK, dV, dOut, q, k, v, out, lse, mask, scale, scratch)
 
     @staticmethod

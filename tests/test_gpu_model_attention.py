@@ -279,3 +279,50 @@ def test_keys_beyond_two_to_the_32_elements(G, rng):
     grads = Tensor.crossAttentionGrad(G.ofNumpy(do), G.ofNumpy(q), mk(64), mk(96), out, lse)
     for g, (ref, bound), what in zip(grads, o.grad(do, G.toNumpy(out), G.toNumpy(lse)), ("d_q", "d_k", "d_v")):
         within(G.toNumpy(g), ref, bound, what)
+
+
+@pytest.mark.parametrize("dt, shape", [(np.float32, (1, 16, 16, 379, 706, 96, 1)), (np.float32, (1, 8, 8, 557, 764, 128, 16)), (np.float32, (1, 8, 8, 120, 2000, 8, 96)),
+                                       (np.float64, (1, 16, 16, 604, 390, 8, 96)), (np.float64, (1, 4, 4, 142, 1171, 128, 8)), (np.float64, (2, 2, 2, 1, 3000, 3, 100))])
+def test_scratch_that_was_asked_for_suffices_for_unlike_widths(G, rng, dt, shape):
+    B, H, Hk, Lq, Lk, Dk, Dv = shape
+    q, k, v, do = inputs(rng, dt, *shape)
+    Q, K, V, DO = (G.ofNumpy(t) for t in (q, k, v, do))
+    scratch = G.zeros([G.scratchBytes("cross_attention", dt, B, H, Hk, Lq, Lk, max(Dk, Dv))], np.uint8)
+    o = Oracle(q, k, v, None, float(dt(1 / np.sqrt(Dk))), unit(dt))
+    out, lse = G.zeros([B, H, Lq, Dv], dt), G.zeros([B, H, Lq], dt)
+    out.FillCrossAttention(Q, K, V, lse=lse, scratch=scratch)
+    within(G.toNumpy(out), o.out, o.out_bound(), "out")
+    grads = [G.zeros(list(t.shape), dt) for t in (q, k, v)]
+    Tensor.FillCrossAttentionGrad(*grads, DO, Q, K, V, out, lse, scratch=scratch)
+    for g, (ref, bound), what in zip(grads, o.grad(do, G.toNumpy(out), G.toNumpy(lse)), ("d_q", "d_k", "d_v")):
+        within(G.toNumpy(g), ref, bound, what)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("Lq, D", [(1, 20), (1, 72), (70, 20), (70, 72), (1, 7)])
+def test_a_key_that_scores_minus_infinity(G, rng, dt, Lq, D):
+    """Such a key has probability 0, at widths that fill no instruction too: what is computed beyond the width must not meet it."""
+    q, k, v, do = inputs(rng, dt, 1, 2, 2, Lq, 45, D, D)
+    q = np.abs(q)                              # an infinity of the keys times any of these is that infinity
+    k[:, :, 7, 0] = k[:, :, 40, 0] = -np.inf
+    mask = np.ones((1, 45), bool)
+    mask[0, [7, 40]] = False                   # the oracle leaves them out
+    o = Oracle(q, k, v, mask, float(dt(1 / np.sqrt(D))), unit(dt))
+    out, lse = Tensor.crossAttention(*(G.ofNumpy(t) for t in (q, k, v)))
+    within(G.toNumpy(out), o.out, o.out_bound(), "out")
+    within(G.toNumpy(lse), o.lse, o.lse_bound(), "lse")
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_masked_keys_have_no_gradient_whatever_is_upstream(G, rng, dt, bad):
+    q, k, v, do = inputs(rng, dt, 2, 2, 1, 40, 90, 24, 24)
+    mask = np.arange(90)[None, :] < np.array([[50], [71]])
+    do[0, 1, 3, 5] = bad
+    Q, K, V, DO, M = (G.ofNumpy(t) for t in (q, k, v, do, mask))
+    out, lse = Tensor.crossAttention(Q, K, V, M)
+    dq, dk, dv = (G.toNumpy(t) for t in Tensor.crossAttentionGrad(DO, Q, K, V, out, lse, M))
+    for t in (dk, dv):
+        assert (t[~np.broadcast_to(mask[:, None], t.shape[:3])] == 0).all()
+        assert np.isfinite(t[1]).all()         # the other sequence is not touched by it
+    assert np.isfinite(dq[1]).all() and np.isfinite(dq[0, 0]).all() and not np.isfinite(dq[0, 1, 3]).any()

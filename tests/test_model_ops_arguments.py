@@ -152,3 +152,22 @@ def test_not_available_on_the_host_device(H):
     from deepnet_amd.tensor import Tensor
     with pytest.raises(NotImplementedError):
         Tensor.embedding(H.ofNumpy(np.zeros((3, 2), F32)), H.ofNumpy(np.zeros(2, I64)))
+
+
+def test_extents_of_attention():
+    """Large work that fits the grids is taken (the query is answered), what does not fit is refused by the query and by the call alike."""
+    lib, n = native.load(), C.c_size_t()
+    assert lib.dnh_cross_attention_scratch_bytes(abi.DNH_F32, 64, 16, 16, 1 << 16, 1 << 16, 64, C.byref(n)) == abi.DNH_OK
+    assert lib.dnh_cross_attention_scratch_bytes(abi.DNH_F32, 128, 64, 64, 1 << 16, 1 << 16, 64, C.byref(n)) == NOT
+    assert lib.dnh_cross_attention_scratch_bytes(abi.DNH_F64, 1 << 40, 1 << 20, 1, 1 << 40, 1 << 40, 64, C.byref(n)) == NOT
+    big = [128, 64, 1 << 16, 4]
+    refused("cross_attention", d(big), None, d(big), d(big), d(big), None, None, None, 0, status=NOT, says="tiles")
+
+
+def test_the_memory_of_a_shared_walk_stays_bounded():
+    """Parts of at most 256 MB: work that fills the chip by itself is not cut into shares for the sake of its end."""
+    lib, n = native.load(), C.c_size_t()
+    for args in ((16, 16, 16, 8000, 1 << 20, 64), (1, 128, 128, 16000, 1 << 18, 128)):
+        native.check(lib.dnh_cross_attention_scratch_bytes(abi.DNH_F32, *args, C.byref(n)))
+        rows = args[0] * args[1] * args[3]
+        assert n.value <= (1 << 28) + rows * 4 * 4
