@@ -169,22 +169,27 @@ template <class T, int DP, int WAVES, bool WHOLE> struct AttStage {
             }
         }
     }
+    // row and first element of the thread's piece j
+    __device__ __forceinline__ int row_of(int j) const { return (threadIdx.x + j * 64 * WAVES) / PER; }
+    __device__ __forceinline__ int elem_of(int j) const { return (threadIdx.x + j * 64 * WAVES - row_of(j) * PER) * N; }
     // rows whose bit is not set, and what lies beyond the width, become zeros
-    __device__ __forceinline__ void store(T* la, T* lb, int Da, int Db, uint32_t word) {
+    __device__ __forceinline__ void clear_off(int Da, int Db, uint32_t word) {
         if (word != ~0u || Da < DP || Db < DP) {
 #pragma unroll
             for (int j = 0; j < NL; j++) {
-                const int i = threadIdx.x + j * 64 * WAVES, r = i / PER, d = (i - r * PER) * N;
-                const bool on = (word >> r) & 1u;
-                if (!on || d >= Da) a[j] = 0;
-                if (!on || d >= Db) b[j] = 0;
+                const bool on = (word >> row_of(j)) & 1u;
+                if (!on || elem_of(j) >= Da) a[j] = 0;
+                if (!on || elem_of(j) >= Db) b[j] = 0;
             }
         }
+    }
+    __device__ __forceinline__ void store(T* la, T* lb, int Da, int Db, uint32_t word) {
+        clear_off(Da, Db, word);
 #pragma unroll
         for (int j = 0; j < NL; j++) {
-            const int i = threadIdx.x + j * 64 * WAVES, r = i / PER, d = (i - r * PER) * N;
-            *(V*)&la[r * kAttPitch<T, DP> + d] = a[j];
-            *(V*)&lb[r * kAttPitch<T, DP> + d] = b[j];
+            const int at = row_of(j) * kAttPitch<T, DP> + elem_of(j);
+            *(V*)&la[at] = a[j];
+            *(V*)&lb[at] = b[j];
         }
     }
 };
@@ -221,12 +226,30 @@ __device__ __forceinline__ int64_t att_row(const AttArgs<T>& p, const Strides4& 
 //
 // Result accumulators: lane row i of accumulator n holds element d_of(n, i) of the width, chosen so that a lane's operands for E
 // accumulators are neighbours in LDS (one read) and its results are neighbours in memory.
-template <class A, int DP> struct AttOps {
+template <class A, int DP, int WAVES = 4, bool WHOLE = true> struct AttOps {
     using Mma = A;
     using T = typename A::T;
     using V = typename Vec16<T>::type;
     using Acc = typename A::Acc;
     static constexpr int M = A::M, N = A::N, GN = A::G * N, NT = DP / GN, NS = kAttTile / M, ND = DP / M, P = kAttPitch<T, DP>;
+    struct Watch {};                                   // (nothing that these instructions could not multiply)
+    static __device__ __forceinline__ bool failed(const Watch&) { return false; }
+    struct __attribute__((aligned(16))) Tile {
+        T x[kAttTile * P];
+    };
+    struct Operand {                                   // a row of the other matrix: element [t][e] is GN t + h N + e
+        V v[NT];
+    };
+    static __device__ __forceinline__ void load(Operand& q, const T* row, int D, int64_t sd, bool vec, int h, Watch&) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) q.v[t] = att_piece<T, WHOLE>(row, GN * t + h * N, D, sd, vec);
+    }
+    static __device__ __forceinline__ void clear(Operand& q) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) q.v[t] = 0;
+    }
+    using Stage = AttStage<T, DP, WAVES, WHOLE>;
+    static __device__ __forceinline__ void store(Stage& st, Tile& a, Tile& b, int Da, int Db, uint32_t word, Watch&) { st.store(a.x, b.x, Da, Db, word); }
     static constexpr int E = ND % N == 0 ? N : ND == 2 ? 2 : 1, NE = ND / E;
     typedef T VE __attribute__((ext_vector_type(E)));
     static __device__ __forceinline__ int d_of(int n, int i) { return (n / E) * (M * E) + E * i + n % E; }
@@ -256,8 +279,10 @@ template <class A, int DP> struct AttOps {
                 if (d < D) row[d * sd] = o[n][r] * f;
             }
     }
-    // s = rows of the tile . x; at: the tile's element [c][h N]
-    static __device__ __forceinline__ void scores(Acc& s, const T* at, const V (&x)[NT]) {
+    // s = rows of sub-tile u . x
+    static __device__ __forceinline__ void scores(Acc& s, const Tile& tile, int u, int c, int h, const Operand& q) {
+        const T* at = tile.x + (u * M + c) * P + h * N;
+        const V(&x)[NT] = q.v;
         V a[2];
         a[0] = *(const V*)at;
         s = 0;
@@ -271,7 +296,10 @@ template <class A, int DP> struct AttOps {
         }
     }
     // two at once
-    static __device__ __forceinline__ void scores(Acc& s, const T* at, const V (&x)[NT], Acc& z, const T* zat, const V (&y)[NT]) {
+    static __device__ __forceinline__ void scores(Acc& s, const Tile& tile, const Operand& q, Acc& z, const Tile& ztile, const Operand& g, int u, int c, int h) {
+        const T *at = tile.x + (u * M + c) * P + h * N, *zat = ztile.x + (u * M + c) * P + h * N;
+        const V(&x)[NT] = q.v;
+        const V(&y)[NT] = g.v;
         V a[2], w[2];
         a[0] = *(const V*)at;
         w[0] = *(const V*)zat;
@@ -305,8 +333,10 @@ template <class A, int DP> struct AttOps {
             else return v[n / E][n % E];
         }
     };
-    // o += (rows of the tile)^T . s for steps [x0, x0 + R) of the tile, s: the sub-tile's registers; first: Row 0 and 1 of those steps
-    static __device__ __forceinline__ void outer(Acc (&o)[ND], const T* at, int x0, int h, const Acc& s) {
+    // o += (rows of sub-tile u)^T . s
+    static __device__ __forceinline__ void outer(Acc (&o)[ND], const Tile& tile, const Acc& s, int u, int c, int h) {
+        const T* at = tile.x + E * c;
+        const int x0 = u * A::R;
         Row a[3];
         a[0].read(at, x0, h);
         a[1].read(at, x0 + 1, h);
@@ -320,7 +350,9 @@ template <class A, int DP> struct AttOps {
         }
     }
     // two at once
-    static __device__ __forceinline__ void outer(Acc (&o)[ND], const T* at, const Acc& s, Acc (&z)[ND], const T* zat, const Acc& y, int x0, int h) {
+    static __device__ __forceinline__ void outer(Acc (&o)[ND], const Tile& tile, const Acc& s, Acc (&z)[ND], const Tile& ztile, const Acc& y, int u, int c, int h) {
+        const T *at = tile.x + E * c, *zat = ztile.x + E * c;
+        const int x0 = u * A::R;
         Row a[2], w[2];
         a[0].read(at, x0, h);
         w[0].read(zat, x0, h);
@@ -341,6 +373,217 @@ template <class A, int DP> struct AttOps {
     }
 };
 
+// ---- the same in single precision on the bf16 matrix instructions ---------------------------------------------------------------------
+// v_mfma_f32_32x32x16_bf16 does in 32 cycles what v_mfma_f32_32x32x2_f32 does in 512.  A float is the exact sum of three bf16 numbers (each
+// the remainder so far, rounded to nearest: 8 + 8 + 8 significant bits), every product of two parts is exact in the instruction, and of the nine
+// partial products the six largest are kept: those dropped are below 2^-23 |a b| together (2 u of one rounded product), and 6 x 32 cycles take
+// the place of 512.  Parts of elements below 2^-109 fall under bf16's smallest denormal: such an element is kept to 2^-134.  An element of
+// 2^127 or more (infinities, NaN) has no such parts: the workgroup that meets one starts again on the float instructions.
+//
+// The instruction's K = 16: lane l supplies A[l % 32][8 (l / 32) + i] and B[8 (l / 32) + i][l % 32], i = 0 .. 7.  Its result lies as that of
+// v_mfma_f32_32x32x2_f32, so registers 8 j .. 8 j + 7 of lane half h are the rows 16 j + 4 h + { 0 .. 3, 8 .. 11 }: with K numbered in this order
+// they are, cut, the B operand of step j of the second product.  Its A operand is the staged tile transposed, four rows of one column a lane:
+// that is what ds_read_b64_tr_b16 delivers (of 16 lanes, lane x supplies the address of row x / 4, columns 4 (x % 4) .. + 3, and gets column x
+// of the four rows), so one copy of the tile serves both products.
+typedef __bf16 Bf8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ void cut2(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+    typedef float F2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{x, y}), B2));
+    x -= __uint_as_float(hi << 16);
+    y -= __uint_as_float(hi & 0xFFFF0000u);
+    mid = __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{x, y}), B2));
+    x -= __uint_as_float(mid << 16);
+    y -= __uint_as_float(mid & 0xFFFF0000u);
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{x, y}), B2));
+}
+template <int DP, int WAVES> struct AttOpsX3 {
+    using Mma = MmaF32;
+    using T = float;
+    using Acc = MmaF32::Acc;
+    using V = Vec16<float>::type;
+    static constexpr int M = 32, NS = 1, ND = DP / 32, NT = DP / 16, P = DP + 8, PLANE = kAttTile * P;
+    typedef uint32_t U2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+    typedef uint16_t H2 __attribute__((ext_vector_type(2)));
+    struct Watch {                                     // the largest first parts, without their signs
+        H2 top = 0;
+        __device__ __forceinline__ void see(uint32_t hi) { top = __builtin_elementwise_max(top, __builtin_bit_cast(H2, hi & 0x7FFF7FFFu)); }
+    };
+    static __device__ __forceinline__ bool failed(const Watch& w) { return w.top[0] >= 0x7F00 || w.top[1] >= 0x7F00; }   // 2^127
+    struct __attribute__((aligned(16))) Tile {
+        uint16_t x[3 * PLANE];
+    };
+    struct Operand {                                   // element [part][t][i] of a row is 16 t + 8 h + i
+        Bf8 v[3][NT];
+    };
+    static __device__ __forceinline__ void cut8(const float (&x)[8], Bf8 (&y)[3], Watch* w) {
+        U4 part[3];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            uint32_t hi, mid, lo;
+            cut2(x[2 * e], x[2 * e + 1], hi, mid, lo);
+            if (w) w->see(hi);
+            part[0][e] = hi;
+            part[1][e] = mid;
+            part[2][e] = lo;
+        }
+#pragma unroll
+        for (int k = 0; k < 3; k++) y[k] = __builtin_bit_cast(Bf8, part[k]);
+    }
+    static __device__ __forceinline__ void load(Operand& q, const float* row, int D, int64_t sd, bool vec, int h, Watch& w) {
+        V f[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) f[t][k] = att_piece<float, true>(row, 16 * t + 8 * h + 4 * k, D, sd, vec);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            float x[8];
+            Bf8 y[3];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = f[t][i / 4][i % 4];
+            cut8(x, y, &w);
+#pragma unroll
+            for (int k = 0; k < 3; k++) q.v[k][t] = y[k];
+        }
+    }
+    static __device__ __forceinline__ void clear(Operand& q) {
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) q.v[k][t] = __builtin_bit_cast(Bf8, U4(0));
+    }
+    using Stage = AttStage<float, DP, WAVES, true>;
+    static __device__ __forceinline__ void store(Stage& st, Tile& a, Tile& b, int Da, int Db, uint32_t word, Watch& w) {
+        st.clear_off(Da, Db, word);
+#pragma unroll
+        for (int j = 0; j < Stage::NL; j++) {
+            const int at = st.row_of(j) * P + st.elem_of(j);
+            auto put3 = [&](uint16_t* t, const V& v) {
+                uint32_t h0, m0, l0, h1, m1, l1;
+                cut2(v[0], v[1], h0, m0, l0);
+                cut2(v[2], v[3], h1, m1, l1);
+                w.see(h0);
+                w.see(h1);
+                *(U2*)(t + at) = U2{h0, h1};
+                *(U2*)(t + at + PLANE) = U2{m0, m1};
+                *(U2*)(t + at + 2 * PLANE) = U2{l0, l1};
+            };
+            put3(a.x, st.a[j]);
+            put3(b.x, st.b[j]);
+        }
+    }
+    static __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0x6); }
+    static __device__ __forceinline__ Acc mfma(const Bf8& a, const Bf8& b, const Acc& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    // c += a . b, the smallest products first
+    static __device__ __forceinline__ void six(Acc& c, const Bf8 (&a)[3], const Bf8& b0, const Bf8& b1, const Bf8& b2) {
+        c = mfma(a[2], b0, c);
+        c = mfma(a[0], b2, c);
+        c = mfma(a[1], b1, c);
+        c = mfma(a[1], b0, c);
+        c = mfma(a[0], b1, c);
+        c = mfma(a[0], b0, c);
+    }
+    static __device__ __forceinline__ void read(Bf8 (&a)[3], const uint16_t* at) {
+#pragma unroll
+        for (int k = 0; k < 3; k++) a[k] = *(const Bf8*)(at + k * PLANE);
+    }
+    // rows at + { 0 .. 3, 8 .. 11 }
+    static __device__ __forceinline__ void read_tr(Bf8 (&a)[3], const uint16_t* at) {
+        typedef short S4 __attribute__((ext_vector_type(4)));
+        typedef short S8 __attribute__((ext_vector_type(8)));
+        typedef __attribute__((address_space(3))) S4* L4;
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            const S4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L4)(at + k * PLANE)), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L4)(at + k * PLANE + 8 * P));
+            a[k] = __builtin_bit_cast(Bf8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+    static __device__ __forceinline__ void scores(Acc& s, const Tile& tile, int, int c, int h, const Operand& q) {
+        const uint16_t* at = tile.x + c * P + 8 * h;
+        Bf8 a[2][3];
+        read(a[0], at);
+        s = 0;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (t + 1 < NT) read(a[(t + 1) & 1], at + 16 * (t + 1));
+            pin();
+            six(s, a[t & 1], q.v[0][t], q.v[1][t], q.v[2][t]);
+            pin();
+        }
+    }
+    static __device__ __forceinline__ void scores(Acc& s, const Tile& tile, const Operand& q, Acc& z, const Tile& ztile, const Operand& g, int, int c, int h) {
+        const uint16_t *at = tile.x + c * P + 8 * h, *zat = ztile.x + c * P + 8 * h;
+        Bf8 a[2][3], w[2][3];
+        read(a[0], at);
+        read(w[0], zat);
+        s = 0;
+        z = 0;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (t + 1 < NT) {
+                read(a[(t + 1) & 1], at + 16 * (t + 1));
+                read(w[(t + 1) & 1], zat + 16 * (t + 1));
+            }
+            pin();
+            six(s, a[t & 1], q.v[0][t], q.v[1][t], q.v[2][t]);
+            six(z, w[t & 1], g.v[0][t], g.v[1][t], g.v[2][t]);
+            pin();
+        }
+    }
+    static __device__ __forceinline__ void outer(Acc (&o)[ND], const Tile& tile, const Acc s, int, int c, int h) {
+        const int x = c & 15;
+        const uint16_t* at = tile.x + (4 * h + (x >> 2)) * P + (c & 16) + 4 * (x & 3);
+        Bf8 a[2][3], y[3];
+        read_tr(a[0], at);
+#pragma unroll
+        for (int k = 0; k < 2 * ND; k++) {
+            const int j = k / ND, m = k + 1;
+            if (k % ND == 0) {
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) e[i] = j ? s[8 + i] : s[i];   // (the constants keep the vector in registers)
+                cut8(e, y, nullptr);
+            }
+            if (m < 2 * ND) read_tr(a[m & 1], at + (m / ND) * 16 * P + (m % ND) * 32);
+            pin();
+            six(o[k % ND], a[k & 1], y[0], y[1], y[2]);
+            pin();
+        }
+    }
+    static __device__ __forceinline__ void outer(Acc (&o)[ND], const Tile& tile, const Acc& s, Acc (&z)[ND], const Tile& ztile, const Acc& y, int u, int c, int h) {
+        outer(o, tile, s, u, c, h);
+        outer(z, ztile, y, u, c, h);
+    }
+    // accumulator n holds elements 32 n .. 32 n + 31
+    static __device__ __forceinline__ void put(float* row, int64_t sd, int D, const Acc (&o)[ND], float f, int h) {
+#pragma unroll
+        for (int n = 0; n < ND; n++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int d = 32 * n + MmaF32::acc_row(4 * g, h);
+                if (d >= D) continue;                  // (widths are whole groups of four)
+                if (sd == 1) {
+                    V v;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = o[n][4 * g + e] * f;
+                    *(V*)(row + d) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) row[(d + e) * sd] = o[n][4 * g + e] * f;
+                }
+            }
+    }
+};
+// What a kernel runs first, and what instead if that fails: the same type where it cannot.
+template <class A, int DP, int WAVES, bool WHOLE> struct AttFirst {
+    typedef AttOps<A, DP, WAVES, WHOLE> Ops;
+};
+template <int DP, int WAVES> struct AttFirst<MmaF32, DP, WAVES, true> {
+    typedef AttOpsX3<DP, WAVES> Ops;
+};
+
 // ---- the softmax of one tile ----------------------------------------------------------------------------------------------------------
 // s: scores S^T of NS sub-tiles, becomes probabilities relative to the running maximum m; l is this lane's share of the sum.  Returns the
 // factor by which what was summed before has to shrink.
@@ -349,7 +592,9 @@ __device__ __forceinline__ typename A::T att_softmax(typename A::Acc (&s)[NS], u
     using T = typename A::T;
     T top = -(T)__builtin_inf();
 #pragma unroll
-    for (int u = 0; u < NS; u++) s[u] *= scale_base;
+    for (int u = 0; u < NS; u++)
+#pragma unroll
+        for (int r = 0; r < A::R; r++) s[u][r] *= scale_base;
     if (word != ~0u) {
 #pragma unroll
         for (int u = 0; u < NS; u++)
@@ -388,33 +633,41 @@ template <class Ops>
 __device__ __forceinline__ void att_store(const AttArgs<typename Ops::T>& p, const typename Ops::Acc (&o)[Ops::ND], uint32_t head, int b, int hk, uint32_t row,
                                           uint32_t split, int h, typename Ops::T m, typename Ops::T l) {
     using T = typename Ops::T;
+    T *to, f;
+    int64_t sd;
     if (p.splits == 1) {
-        Ops::put(p.o + att_row(p, p.so, b, hk, row), p.so.d, p.Dv, o, l == T(0) ? T(0) : T(1) / l, h);   // a row that attends to nothing is zero
+        to = p.o + att_row(p, p.so, b, hk, row);
+        sd = p.so.d;
+        f = l == T(0) ? T(0) : T(1) / l;   // a row that attends to nothing is zero
         if (p.lse_out && h == 0) p.lse_out[att_row(p, p.slse, b, hk, row)] = att_lse_of<typename Ops::Mma>(m, l);
-        return;
+    } else {
+        const size_t at = ((size_t)head * p.rows + row) * p.splits + split;
+        to = p.part_o + at * p.Dv;
+        sd = 1;
+        f = T(1);
+        if (h == 0) {
+            p.part_m[at] = m;
+            p.part_l[at] = l;
+        }
     }
-    const size_t at = ((size_t)head * p.rows + row) * p.splits + split;
-    Ops::put(p.part_o + at * p.Dv, 1, p.Dv, o, T(1), h);
-    if (h == 0) {
-        p.part_m[at] = m;
-        p.part_l[at] = l;
-    }
+    Ops::put(to, sd, p.Dv, o, f, h);
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 // A wavefront owns M rows and keeps their queries in registers; the workgroup's wavefronts share the keys and values, which go through
 // two LDS buffers: the next tile's loads are in flight while this one is worked on, and one barrier per tile suffices (a wavefront
 // that writes buffer b has passed the barrier behind everybody's last reads of it).
-template <class A, int DP, int WAVES, bool WHOLE>
-__global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel(AttArgs<typename A::T> p) {
+template <class Ops> struct AttLds {
+    typename Ops::Tile k[2], v[2];
+    uint32_t words[kAttWords];
+};
+// false: nothing is written, and the workgroup has to take the other instructions
+template <class Ops, int WAVES>
+__device__ __forceinline__ bool att_forward(const AttArgs<typename Ops::T>& p, AttLds<Ops>& lds) {
+    using A = typename Ops::Mma;
     using T = typename A::T;
-    using V = typename Vec16<T>::type;
     using Acc = typename A::Acc;
-    constexpr int M = A::M, N = A::N, GN = A::G * N, NT = DP / GN, NS = kAttTile / M, ND = DP / M, P = kAttPitch<T, DP>;
-    using Ops = AttOps<A, DP>;
-    __shared__ __attribute__((aligned(16))) T Ks[2][kAttTile * P];
-    __shared__ __attribute__((aligned(16))) T Vs[2][kAttTile * P];
-    __shared__ uint32_t words[kAttWords];
+    constexpr int M = A::M, NS = kAttTile / M, ND = Ops::ND;
     uint32_t head, inner;
     att_place(blockIdx.x, p.blocks * p.splits, p.B * p.Hk, &head, &inner);
     const uint32_t block = inner / p.splits, split = inner - block * p.splits;
@@ -422,26 +675,26 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & (M - 1), h = lane / M;
     const uint32_t row = (block * WAVES + wave) * M + c;
     const bool live = row < p.rows;
-    const T* qr = p.q + att_row(p, p.sq, b, hk, live ? row : 0);
-    V q[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) q[t] = att_piece<T, WHOLE>(qr, GN * t + h * N, p.Dk, p.sq.d, p.vec);
+    typename Ops::Watch watch;
+    typename Ops::Operand q;
+    Ops::load(q, p.q + att_row(p, p.sq, b, hk, live ? row : 0), p.Dk, p.sq.d, p.vec, h, watch);
     Acc o[ND];
 #pragma unroll
     for (int i = 0; i < ND; i++) o[i] = 0;
     T m = -(T)__builtin_inf(), l = 0;
+    const T scale_base = p.scale_base;
     const int tiles = (p.Lk + kAttTile - 1) / kAttTile;
     const int t0 = split * p.split_tiles, t1 = tiles < (int)(t0 + p.split_tiles) ? tiles : (int)(t0 + p.split_tiles);
     const T* kb = p.k + b * p.sk.b + hk * p.sk.h;
     const T* vb = p.v + b * p.sv.b + hk * p.sv.h;
-    AttStage<T, DP, WAVES, WHOLE> st;
+    typename Ops::Stage st;
     for (int w0 = t0; w0 < t1; w0 += kAttWords) {
         const int wn = t1 - w0 < kAttWords ? t1 - w0 : kAttWords;
         __syncthreads();
-        att_words(p, b, w0, wn, words, 64 * WAVES);
+        att_words(p, b, w0, wn, lds.words, 64 * WAVES);
         __syncthreads();
         auto next = [&](int i) {   // the next tile that has a key, from i on
-            while (i < wn && __builtin_amdgcn_readfirstlane(words[i]) == 0) i++;
+            while (i < wn && __builtin_amdgcn_readfirstlane(lds.words[i]) == 0) i++;
             return i;
         };
         auto fetch = [&](int i) {
@@ -454,28 +707,50 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel
         int i = next(0), buf = 0;
         if (i < wn) fetch(i);
         while (i < wn) {
-            const uint32_t word = __builtin_amdgcn_readfirstlane(words[i]);
-            st.store(Ks[buf], Vs[buf], p.Dk, p.Dv, word);
+            const uint32_t word = __builtin_amdgcn_readfirstlane(lds.words[i]);
+            Ops::store(st, lds.k[buf], lds.v[buf], p.Dk, p.Dv, word, watch);
             __syncthreads();
             i = next(i + 1);
             if (i < wn) fetch(i);
-            const T *ks = Ks[buf], *vs = Vs[buf];
             Acc s[NS];
+            if constexpr (NS == 1) {
+                Ops::scores(s[0], lds.k[buf], 0, c, h, q);
+            } else {
 #pragma unroll
-            for (int u = 0; u < NS; u++) Ops::scores(s[u], ks + (u * M + c) * P + h * N, q);
-            const T alpha = att_softmax<A, NS>(s, word, h, p.scale_base, m, l);
+                for (int u = 0; u < NS; u++) Ops::scores(s[u], lds.k[buf], u, c, h, q);
+            }
+            const T alpha = att_softmax<A, NS>(s, word, h, scale_base, m, l);
             if (__any(alpha != T(1))) {
 #pragma unroll
                 for (int d = 0; d < ND; d++) o[d] *= alpha;
             }
+            if constexpr (NS == 1) {
+                Ops::outer(o, lds.v[buf], s[0], 0, c, h);
+            } else {
 #pragma unroll
-            for (int u = 0; u < NS; u++) Ops::outer(o, vs + Ops::E * c, u * A::R, h, s[u]);
+                for (int u = 0; u < NS; u++) Ops::outer(o, lds.v[buf], s[u], u, c, h);
+            }
             buf ^= 1;
         }
     }
+    if (!std::is_empty<typename Ops::Watch>::value && __syncthreads_or((int)Ops::failed(watch))) return false;
     l = across_sum<A>(l);
     if (live) att_store<Ops>(p, o, head, b, hk, row, split, h, m, l);
+    return true;
 }
+template <class A, int DP, int WAVES, bool WHOLE>
+__global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel(AttArgs<typename A::T> p) {
+    using First = typename AttFirst<A, DP, WAVES, WHOLE>::Ops;
+    using Exact = AttOps<A, DP, WAVES, WHOLE>;
+    __shared__ union {
+        AttLds<First> first;
+        AttLds<Exact> exact;
+    } lds;
+    if constexpr (!std::is_same<First, Exact>::value)
+        if (att_forward<First, WAVES>(p, lds.first)) return;
+    att_forward<Exact, WAVES>(p, lds.exact);
+}
+
 
 // Few rows (a decoding step): one wavefront takes 16 rows and a share of the keys, straight from memory into the operands' registers.
 // Bound by the bytes of the keys and values: 32 keys at width 64 are 2048 cycles of the matrix pipe and 16 KB, i.e. the pipes keep up with
@@ -642,21 +917,19 @@ template <class A> __device__ __forceinline__ typename A::T att_lse(typename A::
 }
 
 constexpr int kGradWaves = 4;
-template <class T, int DP> struct GradLds {
-    T a[2][kAttTile * kAttPitch<T, DP>];
-    T b[2][kAttTile * kAttPitch<T, DP>];
-    T lse[2][kAttTile], delta[2][kAttTile];
+template <class Ops> struct GradLds {
+    typename Ops::Tile a[2], b[2];
+    typename Ops::T lse[2][kAttTile], delta[2][kAttTile];
     uint32_t words[kAttWords];
 };
 
 // dq: a wavefront owns M rows and walks the keys, as the forward pass does.
-template <class A, int DP, bool WHOLE>
-__device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<typename A::T, DP>& lds, uint32_t at) {
+template <class Ops>
+__device__ __forceinline__ bool att_dq(const AttArgs<typename Ops::T>& p, GradLds<Ops>& lds, uint32_t at) {
+    using A = typename Ops::Mma;
     using T = typename A::T;
-    using V = typename Vec16<T>::type;
     using Acc = typename A::Acc;
-    constexpr int M = A::M, N = A::N, GN = A::G * N, NT = DP / GN, NS = kAttTile / M, ND = DP / M, P = kAttPitch<T, DP>, WAVES = kGradWaves;
-    using Ops = AttOps<A, DP>;
+    constexpr int M = A::M, NS = kAttTile / M, ND = Ops::ND, WAVES = kGradWaves;
     uint32_t head, inner;
     att_place(at, p.blocks * p.splits, p.B * p.Hk, &head, &inner);
     const uint32_t block = inner / p.splits, split = inner - block * p.splits;
@@ -664,14 +937,10 @@ __device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & (M - 1), h = lane / M;
     const uint32_t row = (block * WAVES + wave) * M + c;
     const bool live = row < p.rows;
-    V q[NT], g[NT];
-    const T* qr = p.q + att_row(p, p.sq, b, hk, live ? row : 0);
-    const T* gr = p.d_out + att_row(p, p.sdo, b, hk, live ? row : 0);
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        q[t] = att_piece<T, WHOLE>(qr, GN * t + h * N, p.Dk, p.sq.d, p.vec);
-        g[t] = att_piece<T, WHOLE>(gr, GN * t + h * N, p.Dv, p.sdo.d, p.vec);
-    }
+    typename Ops::Watch watch;
+    typename Ops::Operand q, g;
+    Ops::load(q, p.q + att_row(p, p.sq, b, hk, live ? row : 0), p.Dk, p.sq.d, p.vec, h, watch);
+    Ops::load(g, p.d_out + att_row(p, p.sdo, b, hk, live ? row : 0), p.Dv, p.sdo.d, p.vec, h, watch);
     const T lse = live ? att_lse<A>(p.lse[att_row(p, p.slse, b, hk, row)]) : (T)__builtin_inf();
     const T delta = live ? p.delta[(size_t)head * p.rows + row] : T(0);
     Acc dq[ND];
@@ -681,7 +950,7 @@ __device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<
     const int t0 = split * p.split_tiles, t1 = tiles < (int)(t0 + p.split_tiles) ? tiles : (int)(t0 + p.split_tiles);
     const T* kb = p.k + b * p.sk.b + hk * p.sk.h;
     const T* vb = p.v + b * p.sv.b + hk * p.sv.h;
-    AttStage<T, DP, WAVES, WHOLE> st;
+    typename Ops::Stage st;
     for (int w0 = t0; w0 < t1; w0 += kAttWords) {
         const int wn = t1 - w0 < kAttWords ? t1 - w0 : kAttWords;
         __syncthreads();
@@ -702,15 +971,14 @@ __device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<
         if (i < wn) fetch(i);
         while (i < wn) {
             const uint32_t word = __builtin_amdgcn_readfirstlane(lds.words[i]);
-            st.store(lds.a[buf], lds.b[buf], p.Dk, p.Dv, word);
+            Ops::store(st, lds.a[buf], lds.b[buf], p.Dk, p.Dv, word, watch);
             __syncthreads();
             i = next(i + 1);
             if (i < wn) fetch(i);
-            const T *ks = lds.a[buf], *vs = lds.b[buf];
 #pragma unroll
             for (int u = 0; u < NS; u++) {
                 Acc s, dp;
-                Ops::scores(s, ks + (u * M + c) * P + h * N, q, dp, vs + (u * M + c) * P + h * N, g);
+                Ops::scores(s, lds.a[buf], q, dp, lds.b[buf], g, u, c, h);
 #pragma unroll
                 for (int r = 0; r < A::R; r++) s[r] = A::exp_(s[r] * p.scale_base - lse) * (dp[r] - delta) * p.scale;
                 if (word != ~0u) {
@@ -718,12 +986,13 @@ __device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<
                     for (int r = 0; r < A::R; r++)
                         if (!((word >> (u * M + A::acc_row(r, h))) & 1u)) s[r] = 0;
                 }
-                Ops::outer(dq, ks + Ops::E * c, u * A::R, h, s);
+                Ops::outer(dq, lds.a[buf], s, u, c, h);
             }
             buf ^= 1;
         }
     }
-    if (!live) return;
+    if (!std::is_empty<typename Ops::Watch>::value && __syncthreads_or((int)Ops::failed(watch))) return false;
+    if (!live) return true;
     T* o;
     int64_t sd;
     if (p.splits == 1) {
@@ -734,16 +1003,16 @@ __device__ __forceinline__ void att_dq(const AttArgs<typename A::T>& p, GradLds<
         sd = 1;
     }
     Ops::put(o, sd, p.Dk, dq, T(1), h);
+    return true;
 }
 
 // dk and dv: a wavefront owns M keys and walks the rows of the group's query heads.
-template <class A, int DP, bool WHOLE>
-__device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds<typename A::T, DP>& lds, uint32_t at) {
+template <class Ops>
+__device__ __forceinline__ bool att_dkv(const AttArgs<typename Ops::T>& p, GradLds<Ops>& lds, uint32_t at) {
+    using A = typename Ops::Mma;
     using T = typename A::T;
-    using V = typename Vec16<T>::type;
     using Acc = typename A::Acc;
-    constexpr int M = A::M, N = A::N, GN = A::G * N, NT = DP / GN, NS = kAttTile / M, ND = DP / M, P = kAttPitch<T, DP>, WAVES = kGradWaves;
-    using Ops = AttOps<A, DP>;
+    constexpr int M = A::M, NS = kAttTile / M, ND = Ops::ND, WAVES = kGradWaves;
     uint32_t head, inner;
     att_place(at, p.kblocks * p.ksplits, p.B * p.Hk, &head, &inner);
     const uint32_t block = inner / p.ksplits, split = inner - block * p.ksplits;
@@ -751,18 +1020,15 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & (M - 1), h = lane / M;
     const int key = (block * WAVES + wave) * M + c;
     const bool in = key < p.Lk, on = att_key_on(p, b, key);
-    V k[NT], v[NT];
-    {
-        const T* kr = p.k + b * p.sk.b + hk * p.sk.h + (in ? key : 0) * p.sk.l;
-        const T* vr = p.v + b * p.sv.b + hk * p.sv.h + (in ? key : 0) * p.sv.l;
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            k[t] = att_piece<T, WHOLE>(kr, GN * t + h * N, p.Dk, p.sk.d, p.vec);
-            v[t] = att_piece<T, WHOLE>(vr, GN * t + h * N, p.Dv, p.sv.d, p.vec);
-        }
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-            if (!on) k[t] = v[t] = 0;
+    typename Ops::Watch watch, of_mine;
+    typename Ops::Operand k, v;
+    Ops::load(k, p.k + b * p.sk.b + hk * p.sk.h + (in ? key : 0) * p.sk.l, p.Dk, p.sk.d, p.vec, h, of_mine);
+    Ops::load(v, p.v + b * p.sv.b + hk * p.sv.h + (in ? key : 0) * p.sv.l, p.Dv, p.sv.d, p.vec, h, of_mine);
+    if (on) {
+        watch = of_mine;
+    } else {
+        Ops::clear(k);
+        Ops::clear(v);
     }
     Acc dk[ND], dv[ND];
 #pragma unroll
@@ -770,7 +1036,7 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
     const int tiles = ((int)p.rows + kAttTile - 1) / kAttTile;
     const int t0 = split * p.ksplit_tiles, t1 = tiles < (int)(t0 + p.ksplit_tiles) ? tiles : (int)(t0 + p.ksplit_tiles);
     const bool any = __syncthreads_or((int)on);   // a block whose keys are all masked has nothing to add up
-    AttStage<T, DP, WAVES, WHOLE> st;
+    typename Ops::Stage st;
     T lse = 0, delta = 0;                          // of row threadIdx.x of the tile in flight
     auto fetch = [&](int t) {
         const uint32_t r0 = (uint32_t)t * kAttTile;
@@ -789,18 +1055,17 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
     if (any && t0 < t1) fetch(t0);
     for (int t = t0; any && t < t1; t++) {
         const uint32_t left = p.rows - (uint32_t)t * kAttTile;
-        st.store(lds.a[buf], lds.b[buf], p.Dk, p.Dv, left >= 32 ? ~0u : (1u << left) - 1u);
+        Ops::store(st, lds.a[buf], lds.b[buf], p.Dk, p.Dv, left >= 32 ? ~0u : (1u << left) - 1u, watch);
         if (threadIdx.x < kAttTile) {
             lds.lse[buf][threadIdx.x] = t * kAttTile + threadIdx.x < p.rows ? att_lse<A>(lse) : (T)__builtin_inf();
             lds.delta[buf][threadIdx.x] = delta;
         }
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
-        const T *qs = lds.a[buf], *gs = lds.b[buf];
 #pragma unroll
         for (int u = 0; u < NS; u++) {
             Acc s, dp;
-            Ops::scores(s, qs + (u * M + c) * P + h * N, k, dp, gs + (u * M + c) * P + h * N, v);
+            Ops::scores(s, lds.a[buf], k, dp, lds.b[buf], v, u, c, h);
 #pragma unroll
             for (int r = 0; r < A::R; r++) {
                 const int i = u * M + A::acc_row(r, h);
@@ -808,11 +1073,12 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
                 dp[r] = on ? pr * (dp[r] - lds.delta[buf][i]) * p.scale : T(0);
                 s[r] = pr;
             }
-            Ops::outer(dv, gs + Ops::E * c, s, dk, qs + Ops::E * c, dp, u * A::R, h);
+            Ops::outer(dv, lds.b[buf], s, dk, lds.a[buf], dp, u, c, h);
         }
         buf ^= 1;
     }
-    if (!in) return;
+    if (!std::is_empty<typename Ops::Watch>::value && __syncthreads_or((int)Ops::failed(watch))) return false;
+    if (!in) return true;
     T *ok, *ov;
     int64_t sk, sv;
     if (p.ksplits == 1) {
@@ -832,17 +1098,30 @@ __device__ __forceinline__ void att_dkv(const AttArgs<typename A::T>& p, GradLds
     }
     Ops::put(ok, sk, p.Dk, dk, T(1), h);
     Ops::put(ov, sv, p.Dv, dv, T(1), h);
+    return true;
 }
 
 // Both halves of the backward pass in one launch, so that neither leaves compute units idle while the other runs out: `first` workgroups of
 // dq (dq_first) or of dk and dv, then those of the other.  The half with the longer walks goes first: what is left for the end is short.
 template <class A, int DP, bool WHOLE>
 __global__ __launch_bounds__(64 * kGradWaves, DP <= 64 ? 2 : 1) void attention_grad_kernel(AttArgs<typename A::T> p, uint32_t first, bool dq_first) {
-    __shared__ __attribute__((aligned(16))) GradLds<typename A::T, DP> lds;
+    using First = typename AttFirst<A, DP, kGradWaves, WHOLE>::Ops;
+    using Exact = AttOps<A, DP, kGradWaves, WHOLE>;
+    __shared__ union {
+        GradLds<First> first;
+        GradLds<Exact> exact;
+    } lds;
     const bool front = blockIdx.x < first;
     const uint32_t at = front ? blockIdx.x : blockIdx.x - first;
-    if (front == dq_first) att_dq<A, DP, WHOLE>(p, lds, at);
-    else att_dkv<A, DP, WHOLE>(p, lds, at);
+    if (front == dq_first) {
+        if constexpr (!std::is_same<First, Exact>::value)
+            if (att_dq(p, lds.first, at)) return;
+        att_dq(p, lds.exact, at);
+    } else {
+        if constexpr (!std::is_same<First, Exact>::value)
+            if (att_dkv(p, lds.first, at)) return;
+        att_dkv(p, lds.exact, at);
+    }
 }
 
 // Adds up the shares: workgroups [0, kv) take rows of dk and dv, the others rows of dq; a thread per element.
