@@ -397,12 +397,15 @@ __device__ __forceinline__ void cut2(float x, float y, uint32_t& hi, uint32_t& m
     y -= __uint_as_float(mid & 0xFFFF0000u);
     lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{x, y}), B2));
 }
-template <int DP, int WAVES> struct AttOpsX3 {
+template <int DP, int WAVES, bool PIN> struct AttOpsX3 {
     using Mma = MmaF32;
     using T = float;
     using Acc = MmaF32::Acc;
     using V = Vec16<float>::type;
-    static constexpr int M = 32, NS = 1, ND = DP / 32, NT = DP / 16, P = DP + 8, PLANE = kAttTile * P;
+    static constexpr int M = 32, NS = 1, ND = DP / 32, NT = DP / 16;
+    // LDS rows of 20 or 52 words beyond a multiple of 64: 16 rows' 16-byte reads fall on different banks, and the four rows of a transposed read
+    // overlap little (width 128, 4 words: 355 us of gradient instead of 347).  At width 64 two workgroups have no room for that: 36 words.
+    static constexpr int P = DP == 128 ? 168 : DP + 8, PLANE = kAttTile * P;
     typedef uint32_t U2 __attribute__((ext_vector_type(2)));
     typedef uint32_t U4 __attribute__((ext_vector_type(4)));
     typedef uint16_t H2 __attribute__((ext_vector_type(2)));
@@ -474,7 +477,14 @@ template <int DP, int WAVES> struct AttOpsX3 {
             put3(b.x, st.b[j]);
         }
     }
-    static __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0x6); }
+    // PIN: reads stay ahead of the matrix instructions (as above), which go before the other wavefront's softmax.  Not so in the gradient up to
+    // width 64, which has no registers to read ahead into: 594 us pinned, 560 us as the compiler orders it (16 x 16 heads, 512 queries, 1024 keys).
+    static __device__ __forceinline__ void pin() {
+        if constexpr (PIN) __builtin_amdgcn_sched_barrier(0x6);
+    }
+    template <int P> static __device__ __forceinline__ void hold() {
+        if constexpr (PIN) __builtin_amdgcn_s_setprio(P);
+    }
     static __device__ __forceinline__ Acc mfma(const Bf8& a, const Bf8& b, const Acc& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     // c += a . b, the smallest products first
     static __device__ __forceinline__ void six(Acc& c, const Bf8 (&a)[3], const Bf8& b0, const Bf8& b1, const Bf8& b2) {
@@ -505,6 +515,7 @@ template <int DP, int WAVES> struct AttOpsX3 {
         Bf8 a[2][3];
         read(a[0], at);
         s = 0;
+        hold<1>();
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             if (t + 1 < NT) read(a[(t + 1) & 1], at + 16 * (t + 1));
@@ -512,8 +523,14 @@ template <int DP, int WAVES> struct AttOpsX3 {
             six(s, a[t & 1], q.v[0][t], q.v[1][t], q.v[2][t]);
             pin();
         }
+        hold<0>();
     }
     static __device__ __forceinline__ void scores(Acc& s, const Tile& tile, const Operand& q, Acc& z, const Tile& ztile, const Operand& g, int, int c, int h) {
+        if constexpr (DP <= 64) {                      // (both at once would not fit the registers of two wavefronts a SIMD)
+            scores(s, tile, 0, c, h, q);
+            scores(z, ztile, 0, c, h, g);
+            return;
+        }
         const uint16_t *at = tile.x + c * P + 8 * h, *zat = ztile.x + c * P + 8 * h;
         Bf8 a[2][3], w[2][3];
         read(a[0], at);
@@ -539,6 +556,7 @@ template <int DP, int WAVES> struct AttOpsX3 {
         read_tr(a[0], at);
 #pragma unroll
         for (int k = 0; k < 2 * ND; k++) {
+            hold<1>();
             const int j = k / ND, m = k + 1;
             if (k % ND == 0) {
                 float e[8];
@@ -550,6 +568,7 @@ template <int DP, int WAVES> struct AttOpsX3 {
             pin();
             six(o[k % ND], a[k & 1], y[0], y[1], y[2]);
             pin();
+            if (k % ND == ND - 1) hold<0>();
         }
     }
     static __device__ __forceinline__ void outer(Acc (&o)[ND], const Tile& tile, const Acc& s, Acc (&z)[ND], const Tile& ztile, const Acc& y, int u, int c, int h) {
@@ -577,11 +596,11 @@ template <int DP, int WAVES> struct AttOpsX3 {
     }
 };
 // What a kernel runs first, and what instead if that fails: the same type where it cannot.
-template <class A, int DP, int WAVES, bool WHOLE> struct AttFirst {
+template <class A, int DP, int WAVES, bool WHOLE, bool PIN> struct AttFirst {
     typedef AttOps<A, DP, WAVES, WHOLE> Ops;
 };
-template <int DP, int WAVES> struct AttFirst<MmaF32, DP, WAVES, true> {
-    typedef AttOpsX3<DP, WAVES> Ops;
+template <int DP, int WAVES, bool PIN> struct AttFirst<MmaF32, DP, WAVES, true, PIN> {
+    typedef AttOpsX3<DP, WAVES, PIN> Ops;
 };
 
 // ---- the softmax of one tile ----------------------------------------------------------------------------------------------------------
@@ -740,7 +759,7 @@ __device__ __forceinline__ bool att_forward(const AttArgs<typename Ops::T>& p, A
 }
 template <class A, int DP, int WAVES, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel(AttArgs<typename A::T> p) {
-    using First = typename AttFirst<A, DP, WAVES, WHOLE>::Ops;
+    using First = typename AttFirst<A, DP, WAVES, WHOLE, true>::Ops;
     using Exact = AttOps<A, DP, WAVES, WHOLE>;
     __shared__ union {
         AttLds<First> first;
@@ -1105,7 +1124,7 @@ __device__ __forceinline__ bool att_dkv(const AttArgs<typename Ops::T>& p, GradL
 // dq (dq_first) or of dk and dv, then those of the other.  The half with the longer walks goes first: what is left for the end is short.
 template <class A, int DP, bool WHOLE>
 __global__ __launch_bounds__(64 * kGradWaves, DP <= 64 ? 2 : 1) void attention_grad_kernel(AttArgs<typename A::T> p, uint32_t first, bool dq_first) {
-    using First = typename AttFirst<A, DP, kGradWaves, WHOLE>::Ops;
+    using First = typename AttFirst<A, DP, kGradWaves, WHOLE, (DP > 64)>::Ops;
     using Exact = AttOps<A, DP, kGradWaves, WHOLE>;
     __shared__ union {
         GradLds<First> first;
@@ -1164,14 +1183,15 @@ inline void att_shares(int64_t workgroups, int64_t tiles, int64_t want, int64_t 
     *share_tiles = (uint32_t)each;
 }
 
-// Estimates in microseconds that choose the numbers of shares.  A product of a 32-row tile takes a wavefront DP x 32 cycles of its SIMD's
-// matrix pipe in either precision, at about 2.2 GHz; what else a tile costs it (softmax, staging, a barrier) about 1 us; starting and ending
-// a workgroup 4 us.  Up to padded width 64 two workgroups of four wavefronts fit a compute unit (they share the pipes), above one.
-// Measured with these against a fixed target of 256 workgroups: 80 row blocks at width 128 over 3000 keys 258 -> 199 us forward.
+// Estimates in microseconds that choose the numbers of shares, fitted to 512 queries and 1024 keys at widths 32 to 128: a 32-row tile costs a
+// wavefront 0.0105 us a product and column in single precision and 0.0145 in double precision (matrix instructions, and what cutting, staging and
+// softmax leave uncovered), and 0.3 or 1 us besides; starting and ending a workgroup 4 us.  Up to padded width 64 two workgroups of
+// four wavefronts fit a compute unit (they share the pipes), above one.  Shares chosen so, against a fixed target of 256 workgroups, when the
+// float instructions did the products: 300 queries over 3000 keys at width 128 258 -> 174 us.
 inline int att_resident(int64_t width) { return width <= 64 ? 2 : 1; }
-inline double att_walk_us(int64_t width, int products, int64_t tiles) {
-    const double padded = (double)((width + 31) / 32 * 32);
-    return 4.0 + tiles * (products * padded * 0.0145 * att_resident(width) + 1.0);
+template <class T> double att_walk_us(int64_t width, int products, int64_t tiles) {
+    const double padded = (double)((width + 31) / 32 * 32), column = sizeof(T) == 4 ? 0.0105 : 0.0145, tile = sizeof(T) == 4 ? 0.3 : 1.0;
+    return 4.0 + tiles * (products * padded * column * att_resident(width) + tile);
 }
 // `n` workgroups of `each` us on `slots` places: what a place has to do on average, and half a walk for the uneven end
 inline double att_span_us(double n, double each, double slots) { return n <= slots ? each : n * each / slots + 0.5 * each; }
@@ -1203,7 +1223,7 @@ template <class T> AttPlan att_plan(int64_t heads, int64_t rows, int64_t Lk, int
         for (int64_t n = 1; n <= 64 && (n == 1 || 2 * n <= tiles + 1); n++) {
             const int64_t each = (tiles + n - 1) / n;
             const double bytes = n > 1 ? (double)heads * rows * n * width * sizeof(T) : 0.0;
-            const double us = att_span_us((double)heads * p.blocks * n, att_walk_us(width, 2, each), slots) + att_join_us(bytes);
+            const double us = att_span_us((double)heads * p.blocks * n, att_walk_us<T>(width, 2, each), slots) + att_join_us(bytes);
             if (n > 1 && (us >= best || bytes > kAttPartBytes)) continue;
             best = us;
             p.split_tiles = (uint32_t)(each < 1 ? 1 : each);
@@ -1234,7 +1254,7 @@ template <class T> AttGradPlan att_grad_plan(int64_t heads, int64_t rows, int64_
     for (int64_t n = 1; n <= 64 && (n == 1 || 2 * n <= tk + 1); n = n < 8 ? n + 1 : n + n / 4)
         for (int64_t k = 1; k <= 64 && (k == 1 || 2 * k <= tr + 1); k = k < 8 ? k + 1 : k + k / 4) {
             const int64_t eq = (tk + n - 1) / n, ek = (tr + k - 1) / k;
-            const double uq = att_walk_us(width, 3, eq), uk = att_walk_us(width, 4, ek), longest = uq > uk ? uq : uk;
+            const double uq = att_walk_us<T>(width, 3, eq), uk = att_walk_us<T>(width, 4, ek), longest = uq > uk ? uq : uk;
             const double even = (qn * n * uq + kn * k * uk) / slots + 0.5 * (uq < uk ? uq : uk);
             const double bytes = ((n > 1 ? (double)heads * rows * n : 0.0) + (k > 1 ? (double)heads * Lk * 2 * k : 0.0)) * width * sizeof(T);
             const double us = (qn * n + kn * k <= slots || even < longest ? longest : even) + att_join_us(bytes);

@@ -3,7 +3,8 @@
 Bounds, u half a step of the type, |.| sums of absolute products.  A score is a sum of Dk products (Dk + 1) u S_abs, its scaling and
 the exponent's subtraction add 6 u (|S| + |m|), the exponential 2 u (4 u with its base's constant): every probability before
 normalisation is off by at most r = max over the keys of (Dk + 4) u S_abs + 6 u (|S| + |m|) + 4 u, relatively.  Sums over Lk keys add
-Lk u.  So
+Lk u.  (Where the products of single precision are taken of bf16 parts they are exact but for 2 u of dropped ones; Dk - 1 additions and those
+of the five smaller parts, 5 Dk 2^-8 u, make (Dk + 4) u, too.)  So
   out:  sum_j P_j |v_j| (2 r + (Lk + 16) u)          lse:  r + (Lk + 8) u + 4 u |lse|
 Backward, with out and lse as given: P_j is off by r + 4 u |lse| relatively, dP by (Dv + 2) u (|d_out||v|) and delta by (Dv + 2) u
 (|d_out||out|), dS by e = |dS| (r + 4 u |lse| + 8 u) + scale P (those two); the last product adds (n + 4) u of its absolute sum.
@@ -326,3 +327,37 @@ def test_masked_keys_have_no_gradient_whatever_is_upstream(G, rng, dt, bad):
         assert (t[~np.broadcast_to(mask[:, None], t.shape[:3])] == 0).all()
         assert np.isfinite(t[1]).all()         # the other sequence is not touched by it
     assert np.isfinite(dq[1]).all() and np.isfinite(dq[0, 0]).all() and not np.isfinite(dq[0, 1, 3]).any()
+
+
+@pytest.mark.parametrize("shape", [(1, 4, 2, 70, 150, 16, 24), (1, 2, 2, 40, 333, 64, 64), (1, 1, 1, 130, 90, 128, 128)])
+def test_elements_that_have_no_bf16_parts(G, rng, shape):
+    """Single precision: 2^127 and more, which rounds to an infinity in fewer bits; here in the values, with small upstream gradients."""
+    q, k, v, do = inputs(rng, np.float32, *shape)
+    v[0, 0, 5, 3] = 3e38
+    v[0, -1, -1, 0] = -2e38
+    compare(G, q, k, v, do * np.float32(1e-30))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_a_walk_longer_than_the_mask_words_kept_at_a_time(G, rng, dt):
+    """More sequences than workgroups fit at once, so that each is one walk; they share the same keys and values (a broadcast view)."""
+    B, Lq, Lk, D = 2100, 40, 8300, 4
+    q, k, v, do = inputs(rng, dt, 1, 1, 1, Lq, Lk, D, D)
+    mask = np.ones((B, Lk), bool)
+    mask[:, 100:8200] = False
+    mask[1, :] = False
+    mask[1, 8290:] = True
+    mask[2, :] = False
+    mask[3, :] = True
+    Q, K, V, DO = (G.ofNumpy(t).broadcastTo([B, 1, t.shape[2], D]) for t in (q, k, v, do))
+    M = G.ofNumpy(mask)
+    out, lse = Tensor.crossAttention(Q, K, V, M)
+    dq = G.zeros([B, 1, Lq, D], dt)
+    Tensor.FillCrossAttentionGrad(dq, None, None, DO, Q, K, V, out, lse, M)
+    for b in (0, 1, 2, 3, B - 1):
+        o = Oracle(q, k, v, mask[b:b + 1], float(dt(1 / np.sqrt(D))), unit(dt))
+        go, gl, gq = (G.toNumpy(t[b:b + 1]) for t in (out, lse, dq))
+        within(go, o.out, o.out_bound(), "out")
+        within(gl, o.lse, o.lse_bound(), "lse")
+        ref, bound = o.grad(do, go, gl)[0]
+        within(gq, ref, bound, "d_q")
