@@ -1088,8 +1088,8 @@ __device__ __forceinline__ bool att_dkv(const AttArgs<typename Ops::T>& p, GradL
 #pragma unroll
             for (int r = 0; r < A::R; r++) {
                 const int i = u * M + A::acc_row(r, h);
-                const T pr = on ? A::exp_(s[r] * p.scale_base - lds.lse[buf][i]) : T(0);
-                dp[r] = on ? pr * (dp[r] - lds.delta[buf][i]) * p.scale : T(0);
+                const T pr = A::exp_(s[r] * p.scale_base - lds.lse[buf][i]);   // (a key that is off adds up something, too, which is dropped below)
+                dp[r] = pr * (dp[r] - lds.delta[buf][i]) * p.scale;
                 s[r] = pr;
             }
             Ops::outer(dv, lds.b[buf], s, dk, lds.a[buf], dp, u, c, h);
@@ -1111,7 +1111,7 @@ __device__ __forceinline__ bool att_dkv(const AttArgs<typename Ops::T>& p, GradL
         ov = p.part_dv + at_row * p.Dv;
         sk = sv = 1;
     }
-    if (!on) {   // zero, whatever d_out holds: an infinity there has met the key's zero probabilities
+    if (!on) {
 #pragma unroll
         for (int i = 0; i < ND; i++) dk[i] = dv[i] = 0;
     }
