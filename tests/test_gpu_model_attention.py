@@ -361,3 +361,28 @@ def test_a_walk_longer_than_the_mask_words_kept_at_a_time(G, rng, dt):
         within(gl, o.lse, o.lse_bound(), "lse")
         ref, bound = o.grad(do, go, gl)[0]
         within(gq, ref, bound, "d_q")
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("Lq, H, Hk", [(37, 6, 2), (64, 4, 1), (31, 5, 1)])
+def test_tiles_that_cross_the_heads_of_a_group(G, rng, dt, Lq, H, Hk):
+    """[B; L; H; D] tensors: a tile of 32 rows of a shared key head ends in the next query head, whose rows lie before those of the first one."""
+    q, k, v, do = inputs(rng, dt, 2, H, Hk, Lq, 75, 16, 32)
+    compare(G, q, k, v, do, up=lambda t: G.ofNumpy(np.ascontiguousarray(t.transpose(0, 2, 1, 3))).permuteAxes([0, 2, 1, 3]))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_rows_far_apart(G, rng, dt):
+    """Rows of a tile more than 2^31 bytes apart: keys of every 2^25th element, many query rows."""
+    q, k, v, do = inputs(rng, dt, 1, 1, 1, 50, 40, 32, 32)
+    pitch = 1 << 25
+    cache = Tensor.new([40, pitch], G.Dev, dt)
+    cache[:, 64:96] = G.ofNumpy(k[0, 0])
+    cache[:, 96:128] = G.ofNumpy(v[0, 0])
+    mk = lambda off: cache.Relayout(type(cache.Layout)((1, 1, 40, 32), off, (0, 0, pitch, 1)))
+    out, lse = Tensor.crossAttention(G.ofNumpy(q), mk(64), mk(96))
+    o = Oracle(q, k, v, None, float(dt(1 / np.sqrt(32))), unit(dt))
+    within(G.toNumpy(out), o.out, o.out_bound(), "out")
+    grads = Tensor.crossAttentionGrad(G.ofNumpy(do), G.ofNumpy(q), mk(64), mk(96), out, lse)
+    for g, (ref, bound), what in zip(grads, o.grad(do, G.toNumpy(out), G.toNumpy(lse)), ("d_q", "d_k", "d_v")):
+        within(G.toNumpy(g), ref, bound, what)
