@@ -5,7 +5,7 @@
 //
 // Both are bound by HBM: the lookup reads every row it names and writes N x D, the gradient reads N x D and writes V x D.
 // The gradient needs no atomics: the N token numbers are sorted (stable, with their positions) and each run of equal tokens is added up
-// by one thread per column vector, so the result has the same bits on every run.
+// by one thread per column vector, so the result has the same bits on every run; few tokens are compared with each other instead.
 #include "model_ops.h"
 
 using namespace dnh;
@@ -15,7 +15,9 @@ namespace {
 constexpr int kBlock = 256;
 
 // ---- lookup ---------------------------------------------------------------------------------------------------------------------
-// 2^txl threads share a row (16 bytes each), U rows per thread in flight.
+// 2^txl threads share a row (16 bytes each), U rows per thread in flight.  Bound by HBM: 65 536 rows of 1024 floats from a table of 50 000 are
+// read (rows named twice come from the caches) and written in 59 us, 268 MB of stores alone at 4.6 TB/s; 16 rows take 2.8 us, one
+// memory round trip for the token and one for its row.
 template <class T, bool VEC, int U>
 __global__ __launch_bounds__(kBlock) void embedding_kernel(T* __restrict__ t, const T* __restrict__ table, const int64_t* __restrict__ tokens,
                                                            RowPlan<2> rp, uint32_t n, int64_t td, int64_t tab_row, int64_t tab_d, int64_t vocab,
@@ -82,7 +84,9 @@ int32_t launch_embedding(const DnhTensor* t, const DnhTensor* table, const DnhTe
 // ---- sorting the tokens ------------------------------------------------------------------------------------------------------------
 // Stable least-significant-digit radix sort of (token, position).  A token outside the table gets the key `vocab` and ends up behind
 // all others, where nothing reads it.  Ranks come from ballots: lanes of a wavefront that share a digit find each other with one ballot
-// per digit bit; each wavefront counts its own digits in LDS while it walks its part of the tile in order.
+// per digit bit; each wavefront counts its own digits in LDS while it walks its part of the tile in order.  Bound by latency (barriers and
+// dependent LDS accesses), not by bytes: 4095 tokens of 14 bits take one launch of 13 us, 32 768 of 16 bits two pairs of 6 + 13 us, in which
+// the target is cleared besides (205 MB).  Up to 8192 tokens one workgroup is faster than a pair of launches for each digit.
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kMinDigitBits = 6, kMaxDigitBits = 9, kMaxDigits = 1 << kMaxDigitBits;
 constexpr uint32_t kSmallSort = 8192;    // tokens that one workgroup sorts in LDS, in one launch
@@ -339,7 +343,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(TokenSource sr
 // ---- adding up the runs --------------------------------------------------------------------------------------------------------------
 // The sorted list is cut into pieces of R entries; 2^txl threads take a piece, 16 bytes of the row each, and add in 64 bits.  A run
 // inside the piece goes straight to its row of the target.  The part of a run that began in an earlier piece goes to the piece's first
-// partial, the part of a run that goes on behind it to its second one; the second kernel adds those.
+// partial, the part of a run that goes on behind it to its second one; the second kernel adds those.  Bound by the reads of d_out, a row at
+// a time in the tokens' order, eight in flight: 32 768 x 1024 floats (134 MB, part of it from the 256 MB cache) in 32 us.
 template <class T> struct GradTarget {
     T* t;
     int64_t row_stride, d_stride, width;
@@ -426,7 +431,7 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(GradTarget<T> tg,
 }
 
 // Runs that cross pieces.  The workgroups of the piece in which such a run begins add its partials: 256 columns each, the pieces dealt
-// to four wavefronts, whose sums are added in order.
+// to four wavefronts, whose sums are added in order.  The longest run decides: token frequencies of 1 / rank, 32 768 tokens, 10 us.
 constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kJoinCols = 256;
 template <class T>
 __global__ __launch_bounds__(kJoinThreads) void embedding_join_kernel(GradTarget<T> tg, const uint32_t* __restrict__ keys, uint32_t n, uint32_t vocab, uint32_t R,
@@ -467,6 +472,128 @@ __global__ __launch_bounds__(kJoinThreads) void embedding_join_kernel(GradTarget
         double v = 0;
         for (int w = 0; w < kJoinWaves; w++) v += sums[w][threadIdx.x];
         put(tg, key, c, v);
+    }
+}
+
+// ---- few tokens -----------------------------------------------------------------------------------------------------------------------
+// Up to kFewTokens everything in one launch, without a sort: each workgroup reads all the tokens.  Those of leader i add up the rows of the
+// tokens equal to the i-th unless one before it is equal, 16 bytes of the row per lane, equal tokens dealt to four wavefronts whose sums
+// are added in order.  The others clear blocks of rows, leaving out those that a leader writes.  Bound by latency: the tokens, the rows, the sums.
+// 512 tokens into 10 007 rows of 300 floats 8.6 us against 15.7 us sorted (513 tokens), 16 tokens 7.6 us; into 50 000 rows of 1024 (205 MB to
+// clear) 40 us against 47; 500 tokens into 500 rows of 2000, where the sums are most of it, 12.4 us against 14.3.
+constexpr uint32_t kFewTokens = 512;
+constexpr int kFillRows = 2048;   // most rows of a block that is cleared at once
+bool few_tokens(int64_t n, int64_t width) { return n <= kFewTokens && n * width <= (1 << 28); }   // (a grid of fewer than 2^32 threads for any width)
+template <class T, bool VEC>
+__global__ __launch_bounds__(kBlock) void embedding_grad_few_kernel(GradTarget<T> tg, TokenSource src, const T* __restrict__ g, RowPlan<1> gp, int64_t gd, uint32_t chunks,
+                                                                    uint32_t block_rows, int txl) {
+    constexpr int N = VEC ? kVecN<T> : 1, U = 8, COLS = 64 * N, WAVES = kBlock / 64, PER = kFewTokens / WAVES;
+    using V = typename Vec16<T>::type;
+    __shared__ uint32_t keys[kFewTokens];
+    __shared__ uint32_t list[kFewTokens];
+    __shared__ uint32_t counts[WAVES];
+    __shared__ uint32_t marks[kFillRows / 32];
+    __shared__ double sums[WAVES][COLS];
+    const uint32_t n = src.n;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (uint32_t i = threadIdx.x; i < kFewTokens; i += kBlock) keys[i] = i < n ? token_key(src, i) : src.vocab;
+    __syncthreads();
+    if (blockIdx.x >= n * chunks) {
+        const uint32_t wg = blockIdx.x - n * chunks, wgs = gridDim.x - n * chunks;
+        const int per = kBlock >> txl, sub = threadIdx.x >> txl, col = threadIdx.x & ((1 << txl) - 1);
+        constexpr int NZ = kVecN<T>;
+        for (uint64_t r0 = (uint64_t)wg * block_rows; r0 < src.vocab; r0 += (uint64_t)wgs * block_rows) {
+            if (threadIdx.x < kFillRows / 32) marks[threadIdx.x] = 0;
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < n; i += kBlock)
+                if (keys[i] >= r0 && keys[i] < r0 + block_rows && keys[i] != src.vocab) atomicOr(&marks[(keys[i] - (uint32_t)r0) >> 5], 1u << ((keys[i] - (uint32_t)r0) & 31));
+            __syncthreads();
+            for (uint32_t r = sub; r < block_rows && r0 + r < src.vocab; r += per) {
+                if ((marks[r >> 5] >> (r & 31)) & 1u) continue;
+                T* row = tg.t + (int64_t)(r0 + r) * tg.row_stride;
+                for (int64_t c = (int64_t)col * NZ; c < tg.width; c += (int64_t)NZ << txl) {
+                    if (tg.d_stride == 1 && c + NZ <= tg.width) {
+                        __builtin_nontemporal_store(V(0), (V*)(row + c));
+                    } else {
+                        for (int64_t e = c; e < c + NZ && e < tg.width; e++) row[e * tg.d_stride] = T(0);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        return;
+    }
+    const uint32_t leader = blockIdx.x / chunks, key = keys[leader];
+    // the list of equal tokens, in order: each wavefront finds those of its quarter
+    uint32_t at[PER / 64], mine = 0;
+    bool is[PER / 64], before = false;
+#pragma unroll
+    for (int e = 0; e < PER / 64; e++) {
+        const uint32_t j = wave * PER + e * 64 + lane;
+        is[e] = j < n && keys[j] == key;
+        before |= is[e] && j < leader;
+        const unsigned long long m = __ballot(is[e]);
+        at[e] = mine + (uint32_t)__popcll(m & ((1ull << lane) - 1ull));
+        mine += (uint32_t)__popcll(m);
+    }
+    if (lane == 0) counts[wave] = mine;
+    if (__syncthreads_or((int)(before || key == src.vocab))) return;   // an equal token before it, or none of the table
+    uint32_t first = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        if (w < wave) first += counts[w];
+        total += counts[w];
+    }
+#pragma unroll
+    for (int e = 0; e < PER / 64; e++)
+        if (is[e]) list[first + at[e]] = wave * PER + e * 64 + lane;
+    __syncthreads();
+    const int64_t c = (int64_t)(blockIdx.x - leader * chunks) * COLS + lane * N;
+    const int live = c >= tg.width ? 0 : (int)(tg.width - c < N ? tg.width - c : N);
+    double acc[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) acc[e] = 0;
+    for (uint32_t k = wave; k < total; k += U * WAVES) {
+        T x[U][N];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t q = k + u * WAVES;
+            int64_t off[1];
+            row_offsets(gp, list[q < total ? q : total - 1], off);
+            const T* p = g + off[0];
+            if (VEC && live == N) {
+                const V v = *(const V*)(p + c);
+#pragma unroll
+                for (int e = 0; e < N; e++) x[u][e] = v[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; e++) x[u][e] = e < live ? p[(c + e) * gd] : T(0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (k + u * WAVES < total) {
+#pragma unroll
+                for (int e = 0; e < N; e++) acc[e] += (double)x[u][e];
+            }
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++) sums[wave][lane * N + e] = acc[e];
+    __syncthreads();
+    if (wave != 0 || live == 0) return;
+    const int others = total < (uint32_t)WAVES ? (int)total : WAVES;
+    for (int w = 1; w < others; w++)
+#pragma unroll
+        for (int e = 0; e < N; e++) acc[e] += sums[w][lane * N + e];
+    if (VEC && live == N && tg.d_stride == 1) {
+        V* p = (V*)(tg.t + (int64_t)key * tg.row_stride + c);
+        V v = 0;
+        if (tg.accumulate) v = *p;
+#pragma unroll
+        for (int e = 0; e < N; e++) v[e] = (T)((double)v[e] + acc[e] * tg.scale);
+        *p = v;
+    } else {
+        for (int e = 0; e < live; e++) put(tg, key, c + e, acc[e]);
     }
 }
 
@@ -514,14 +641,25 @@ int32_t embedding_grad(const DnhTensor* dt, const DnhTensor* tokens, const DnhTe
     char* ws = nullptr;
     WorkspaceLease lease;
     DNH_TRY(error_flag_ptr(s, &src.err));
+    // (few tokens use none of it; the call's contract, above all what a captured call has to bring, is the same at every size)
     DNH_TRY(get_scratch(s, n ? p.total : 0, scratch, scratch_bytes, (void**)&ws, lease, "dnh_embedding_grad"));
-    const unsigned fill_wgs = accumulate ? 0 : (unsigned)(2 * device_cus());
-    if (n == 0) {
-        if (accumulate) return DNH_OK;
-        hipLaunchKernelGGL((sort_small_kernel<T, 1>), dim3(1 + fill_wgs), dim3(kSortThreads), 0, s, src, 0, kMinDigitBits, nullptr, nullptr, z);
+    const RowPlan<1> gp = make_row_plan<1>(nd, {d_out});
+    const bool vec = d_out->stride[nd] == 1;
+    if (few_tokens(n, width)) {
+        const unsigned chunks = cdiv(width, 64 * (vec ? kVecN<T> : 1));
+        // blocks of 16 to 32 KB, a workgroup each until there are eight per compute unit
+        uint32_t block_rows = 1;
+        while (block_rows < kFillRows && (int64_t)block_rows * width * (int64_t)sizeof(T) < (1 << 14)) block_rows *= 2;
+        const int64_t blocks = accumulate ? 0 : ((int64_t)vocab + block_rows - 1) / block_rows, most = 8 * (int64_t)device_cus();
+        const unsigned grid = n * chunks + (unsigned)(blocks < most ? blocks : most);
+        const int txl = lanes_log2((width + kVecN<T> - 1) / kVecN<T>);
+        if (grid == 0) return DNH_OK;
+        if (vec) hipLaunchKernelGGL((embedding_grad_few_kernel<T, true>), dim3(grid), dim3(kBlock), 0, s, tg, src, (const T*)elem_ptr(d_out), gp, d_out->stride[nd], chunks, block_rows, txl);
+        else hipLaunchKernelGGL((embedding_grad_few_kernel<T, false>), dim3(grid), dim3(kBlock), 0, s, tg, src, (const T*)elem_ptr(d_out), gp, d_out->stride[nd], chunks, block_rows, txl);
         DNH_LAUNCH_CHECK();
         return DNH_OK;
     }
+    const unsigned fill_wgs = accumulate ? 0 : (unsigned)(2 * device_cus());
     uint32_t* list[2][2];   // [buffer][keys, positions]
     for (int b = 0; b < 2; b++)
         for (int k = 0; k < 2; k++) list[b][k] = (uint32_t*)(ws + (n <= kSmallSort ? k : 2 * b + k) * p.list_bytes);
@@ -559,8 +697,6 @@ int32_t embedding_grad(const DnhTensor* dt, const DnhTensor* tokens, const DnhTe
         }
     }
     const uint32_t *keys = list[cur][0], *pos = list[cur][1];
-    const RowPlan<1> gp = make_row_plan<1>(nd, {d_out});
-    const bool vec = d_out->stride[nd] == 1;
     const int64_t items = vec ? (width + kVecN<T> - 1) / kVecN<T> : width;
     const int txl = lanes_log2(items);
     const dim3 grid(cdiv(p.pieces, kBlock >> txl), cdiv(items, (int64_t)1 << txl));

@@ -243,7 +243,7 @@ __device__ __forceinline__ float larger(float x, float y) {
 __device__ __forceinline__ double larger(double x, double y) { return y > x || x != x ? y : x; }
 
 // U x N elements at once.  Single precision is bound by instructions if every term goes to double precision by itself (28 cycles of 4 per
-// element, 155 us for 4096 rows of 50 048, against 126 us for the bytes), so groups of U x N are added up in 32 bits first, five roundings
+// element, 155 us for 4096 rows of 50 048 without alternatives, against 127 us as it is), so groups of U x N are added up in 32 bits first, five roundings
 // deep.  That would lose the rest beside a dominant logit, whose term is exactly 1: the ones are kept out of the sum (v_fract_f32 turns 1
 // into 0 and leaves what is below 1) and counted by the difference of the sums with and without them, which is a whole number
 // up to a rounding.
@@ -284,6 +284,9 @@ __device__ __forceinline__ double shrink(double d, float) {
 __device__ __forceinline__ double shrink(double d, double) { return exp(d); }
 
 // A workgroup takes elements [j0, j1) of a row.  With one workgroup per row it writes the results, else its statistics and list.
+// Without alternatives it runs at the memory's rate: 4096 rows of 50 048 floats (820 MB) in 127 us, 6.5 TB/s.  With 5 alternatives 149 us: sorting
+// the start of a row and inserting what passes the floor later take turns with the loads of the same wavefront.  One row of 128 000 with 20
+// alternatives is a chain of latencies: 32 slices in 11 us, joined in 9 us.
 template <class T, bool VEC, bool TOP>
 __global__ __launch_bounds__(kBlock, TOP ? 5 : 1) void log_probs_kernel(LogProbArgs<T> p, uint32_t splits, uint32_t slice, Stats* __restrict__ part_st, T* __restrict__ part_v,
                                                            uint32_t* __restrict__ part_i) {
@@ -510,7 +513,8 @@ __device__ __forceinline__ T grad_of(T x, T lse, T H, T g, T h) {
     else return -(g * p);
 }
 
-// A workgroup takes U x 16 bytes per thread of a row.
+// A workgroup takes U x 16 bytes per thread of a row, straight through: 4096 rows of 50 048 floats are read and written (1.64 GB) in 265 us,
+// 6.2 TB/s, what a copy reaches.  Double precision is bound by its exponential: 333 rows of 32 003 in 31 us, 5.6 TB/s of 171 MB from the cache.
 template <class T, bool VEC, bool ENT>
 __global__ __launch_bounds__(kBlock) void log_probs_grad_kernel(GradArgs<T> p) {
     constexpr int N = VEC ? kVecN<T> : 1, U = 4;

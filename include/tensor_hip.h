@@ -344,8 +344,8 @@ int32_t dnh_symmetric_eig(int32_t part, const DnhTensor* eigvals, const DnhTenso
  * rounded once.  A token outside the table sets the stream's error flag (dnh_async_error) and leaves its row of t unwritten. */
 int32_t dnh_embedding(const DnhTensor* t, const DnhTensor* table, const DnhTensor* tokens_i64, const void* scale, void* stream);
 /* d_table[v, :] = scale * sum of d_out[i, :] over the i with tokens[i] = v, for every row v (accumulate = 0: rows of absent tokens
- * become zero), or that sum added to d_table (accumulate = 1: rows of absent tokens stay untouched).  The tokens are sorted and each
- * row's addends summed in double precision, in an order that depends on the tokens alone; one rounding at the end.  A token outside
+ * become zero), or that sum added to d_table (accumulate = 1: rows of absent tokens stay untouched).  Each row's
+ * addends are summed in double precision, in an order that depends on the tokens alone; one rounding at the end.  A token outside
  * the table sets the stream's error flag and contributes nothing.  Up to 2^27 tokens. */
 int32_t dnh_embedding_grad(const DnhTensor* d_table, const DnhTensor* tokens_i64, const DnhTensor* d_out, const void* scale, int32_t accumulate,
                            void* scratch, size_t scratch_bytes, void* stream);
@@ -374,7 +374,9 @@ int32_t dnh_token_log_probs_grad(const DnhTensor* d_logits, const DnhTensor* log
  * q [B; Hq; Lq; Dk], k [B; Hk; Lk; Dk], v [B; Hk; Lk; Dv], out [B; Hq; Lq; Dv], lse [B; Hq; Lq] or NULL.  Hq is a multiple of Hk: query
  * head h reads key head h / (Hq / Hk).  mask [B; Lk] (bool) or NULL: keys with false are not attended to, and what k and v hold there
  * (infinities and NaN included) is not used.  A sequence without keys has out 0 and lse -inf.  scale defaults to 1 / sqrt(Dk).
- * Widths up to 128.  [B; L; H; D] tensors are passed as permuted views. */
+ * Widths up to 128.  [B; L; H; D] tensors are passed as permuted views.  Single precision: where widths are multiples of 4 along contiguous
+ * axes the products are taken on the bf16 matrix instructions from three parts of every number, with the error of a float product; elements
+ * below 2^-109 are kept to 2^-134 there, elements of 2^127 and more (and infinities) take the float instructions. */
 int32_t dnh_cross_attention(const DnhTensor* out, const DnhTensor* lse, const DnhTensor* q, const DnhTensor* k, const DnhTensor* v,
                             const DnhTensor* mask_bool, const void* scale, void* scratch, size_t scratch_bytes, void* stream);
 /* Gradients of sum(d_out out) with out and lse as dnh_cross_attention gave them: d_q like q, d_k like k, d_v like v, those of a shared key

@@ -386,3 +386,12 @@ def test_rows_far_apart(G, rng, dt):
     grads = Tensor.crossAttentionGrad(G.ofNumpy(do), G.ofNumpy(q), mk(64), mk(96), out, lse)
     for g, (ref, bound), what in zip(grads, o.grad(do, G.toNumpy(out), G.toNumpy(lse)), ("d_q", "d_k", "d_v")):
         within(G.toNumpy(g), ref, bound, what)
+
+
+def test_elements_whose_last_part_is_a_denormal(G, rng):
+    """One key: out is its value.  Below 2^-109 the last of three bf16 parts has bits under 2^-133, the least bf16 has: off by half of it."""
+    q, k, v, do = inputs(rng, np.float32, 1, 1, 1, 70, 1, 64, 64)
+    v *= np.exp2(rng.integers(-120, -105, v.shape)).astype(np.float32)
+    out, _ = Tensor.crossAttention(*(G.ofNumpy(t) for t in (q, k, v)))
+    err = np.abs(G.toNumpy(out).astype(np.float64) - v[:, :, :1])
+    assert (err <= 2.0 ** -134 + 2 * 2.0 ** -24 * np.abs(v[:, :, :1])).all()

@@ -172,3 +172,18 @@ def test_rows_beyond_two_to_the_32_elements(G):
         np.testing.assert_array_equal(G.toNumpy(table[int(t)]), rows[i])
     assert not G.toNumpy(table[vocab - 4]).any() and not G.toNumpy(table[(1 << 22) - 1]).any()
     assert float(table.sum()) == float(G.ofNumpy(rows).sum())
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n,vocab,width", [(512, 3000, 20), (513, 3000, 20), (257, 70000, 1), (500, 1200, 1030), (512, 1, 300), (300, 5000, 64), (1024, 700, 30)])
+def test_gradient_of_few_tokens(G, rng, dt, n, vocab, width):
+    """Around the number up to which one launch does it all: many blocks of rows to clear, one token named by every position, rows in several
+    pieces, read and written along another axis too."""
+    tok = zipf(rng, n, vocab) if vocab > 1 else np.zeros(n, np.int64)
+    g = rng.standard_normal((n, width)).astype(dt)
+    d = G.filled([vocab, width], dt(np.nan), dt)
+    d.FillEmbeddingGrad(G.ofNumpy(tok), G.ofNumpy(g))
+    check_grad(G.toNumpy(d), tok, g, vocab, 1.0)
+    d = G.filled([width, vocab], dt(np.nan), dt)
+    d.T.FillEmbeddingGrad(G.ofNumpy(tok), G.ofNumpy(np.ascontiguousarray(g.T)).T, 0.3)
+    check_grad(np.ascontiguousarray(G.toNumpy(d).T), tok, g, vocab, 0.3)
