@@ -736,23 +736,15 @@ __device__ __forceinline__ bool att_forward(const AttArgs<typename Ops::T>& p, A
             i = next(i + 1);
             if (i < wn) fetch(i);
             Acc s[NS];
-            if constexpr (NS == 1) {
-                Ops::scores(s[0], lds.k[buf], 0, c, h, q);
-            } else {
 #pragma unroll
-                for (int u = 0; u < NS; u++) Ops::scores(s[u], lds.k[buf], u, c, h, q);
-            }
+            for (int u = 0; u < NS; u++) Ops::scores(s[u], lds.k[buf], u, c, h, q);
             const T alpha = att_softmax<A, NS>(s, word, h, scale_base, m, l);
             if (__any(alpha != T(1))) {
 #pragma unroll
                 for (int d = 0; d < ND; d++) o[d] *= alpha;
             }
-            if constexpr (NS == 1) {
-                Ops::outer(o, lds.v[buf], s[0], 0, c, h);
-            } else {
 #pragma unroll
-                for (int u = 0; u < NS; u++) Ops::outer(o, lds.v[buf], s[u], u, c, h);
-            }
+            for (int u = 0; u < NS; u++) Ops::outer(o, lds.v[buf], s[u], u, c, h);
             buf ^= 1;
         }
     }
