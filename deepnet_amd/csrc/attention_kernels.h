@@ -771,7 +771,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel
 // Bound by the bytes of the keys and values: 32 keys at width 64 are 2048 cycles of the matrix pipe and 16 KB, i.e. the pipes keep up with
 // three times the memory's rate.  A lane of value row `key` loads elements 16-byte-wise and uses element e of load g for
 // accumulator E g + e: accumulator i holds the elements E 16 g + E row + e of the result.
-// 16 sequences of up to 2000 keys, 4 key heads at width 64 (47 MB): 12.7 to 14.7 us, and 4.6 us for joining the shares.  The float instructions
+// 16 sequences of up to 2000 keys, 4 key heads at width 64 (47 MB): 12.7 to 14.7 us, and 4.4 us for joining the shares.  The float instructions
 // stay here: cutting a tile that one wavefront uses once costs more than it saves.
 template <class A, int DP, bool WHOLE>
 __global__ __launch_bounds__(64) void attention_few_kernel(AttArgs<typename A::T> p) {
@@ -873,40 +873,60 @@ __global__ __launch_bounds__(64) void attention_few_kernel(AttArgs<typename A::T
     if (live) att_store<AttOps<A, DP>>(p, o, head, b, hk, row, split, h, m, l);   // (E = N there, too: the same elements in the same accumulators)
 }
 
-// Joins the shares of each row: a wavefront per row, first the shares' weights across its lanes, then lanes along the width.  A launch and two
-// dependent reads: 4.6 us for 256 rows of 32 shares.
-template <class A>
+// Joins the shares of each row, first their weights across the lanes, then lanes along the width: a wavefront per row or, with many shares, the
+// four of a workgroup, whose sums are added in order.  A launch and two dependent reads: 4.4 us for 256 rows of 32 shares (a wavefront each 5.5).
+// One query of a long sequence needs many shares: 100 000 keys of 2 heads at width 64 take 38 us with 256 shares, 101 us with 64.
+constexpr uint32_t kMaxShares = 256;
+template <class A, bool WIDE>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs<typename A::T> p) {
     using T = typename A::T;
-    __shared__ T weights[4][64];
+    __shared__ T weights[4][kMaxShares];
+    __shared__ T sums[4][128];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const size_t row = (size_t)blockIdx.x * 4 + wave;
-    if (row >= (size_t)p.B * p.Hk * p.rows) return;   // (no barrier below: a wavefront uses its own weights only)
+    const size_t row = WIDE ? blockIdx.x : (size_t)blockIdx.x * 4 + wave;
+    if (row >= (size_t)p.B * p.Hk * p.rows) return;   // (a whole workgroup or, with no barrier below, a wavefront)
     const uint32_t head = (uint32_t)(row / p.rows), r = (uint32_t)(row - (size_t)head * p.rows);
     const int b = head / p.Hk, hk = head - b * p.Hk;
-    const bool in = (uint32_t)lane < p.splits;         // at most 64 shares
-    const T pm = in ? p.part_m[row * p.splits + lane] : -(T)__builtin_inf(), pl = in ? p.part_l[row * p.splits + lane] : T(0);
-    T m = pm;
+    constexpr int K = kMaxShares / 64;
+    T pm[K], pl[K], m = -(T)__builtin_inf(), l = 0;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const uint32_t s = k * 64 + lane;
+        pm[k] = s < p.splits ? p.part_m[row * p.splits + s] : -(T)__builtin_inf();
+        pl[k] = s < p.splits ? p.part_l[row * p.splits + s] : T(0);
+    }
+#pragma unroll
+    for (int k = 0; k < K; k++) m = pm[k] > m ? pm[k] : m;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const T y = __shfl_xor(m, d);
         m = y > m ? y : m;
     }
-    const T w = A::exp_(pm - (m == -(T)__builtin_inf() ? T(0) : m));
-    T l = w * pl;
+    const T mu = m == -(T)__builtin_inf() ? T(0) : m;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const T w = A::exp_(pm[k] - mu);              // (0 beyond the last share)
+        weights[wave][k * 64 + lane] = w;
+        l += w * pl[k];
+    }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
-    weights[wave][lane] = l == T(0) ? T(0) : w / l;
-    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_wave_barrier();                  // (a wavefront uses its own weights only)
+    const T f = l == T(0) ? T(0) : T(1) / l;
     T* orow = p.o + att_row(p, p.so, b, hk, r);
     const T* part = p.part_o + row * p.splits * p.Dv;
     for (int d = lane; d < p.Dv; d += 64) {
         T o = 0;
 #pragma unroll 8
-        for (uint32_t s = 0; s < p.splits; s++) o += weights[wave][s] * part[(size_t)s * p.Dv + d];
-        orow[d * p.so.d] = o;
+        for (uint32_t s = WIDE ? wave : 0; s < p.splits; s += WIDE ? 4 : 1) o += weights[wave][s] * part[(size_t)s * p.Dv + d];
+        if (WIDE) sums[wave][d] = o;
+        else orow[d * p.so.d] = o * f;
     }
-    if (p.lse_out && lane == 0) p.lse_out[att_row(p, p.slse, b, hk, r)] = att_lse_of<A>(m, l);
+    if (WIDE) {
+        __syncthreads();
+        for (int d = threadIdx.x; d < p.Dv; d += 256) orow[d * p.so.d] = (((sums[0][d] + sums[1][d]) + sums[2][d]) + sums[3][d]) * f;
+    }
+    if (p.lse_out && lane == 0 && (!WIDE || wave == 0)) p.lse_out[att_row(p, p.slse, b, hk, r)] = att_lse_of<A>(m, l);
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------------------------
@@ -1217,13 +1237,13 @@ template <class T> AttPlan att_plan(int64_t heads, int64_t rows, int64_t Lk, int
     if (rows <= kFewRows) {
         p.waves = 0;
         p.blocks = cdiv(rows, 16);
-        att_shares(heads * p.blocks, tiles, 8 * kAttCUs, 64, &p.splits, &p.split_tiles);    // two wavefronts per SIMD
+        att_shares(heads * p.blocks, tiles, 8 * kAttCUs, kMaxShares, &p.splits, &p.split_tiles);    // two wavefronts per SIMD
     } else {
         p.waves = rows <= 2 * M ? 2 : 4;
         p.blocks = cdiv(rows, (int64_t)p.waves * M);
         const double slots = (double)kAttCUs * att_resident(width) * 4 / p.waves;
         double best = 0;
-        for (int64_t n = 1; n <= 64 && (n == 1 || 2 * n <= tiles + 1); n++) {
+        for (int64_t n = 1; n <= kMaxShares && (n == 1 || 2 * n <= tiles + 1); n++) {
             const int64_t each = (tiles + n - 1) / n;
             const double bytes = n > 1 ? (double)heads * rows * n * width * sizeof(T) : 0.0;
             const double us = att_span_us((double)heads * p.blocks * n, att_walk_us<T>(width, 2, each), slots) + att_join_us(bytes);
@@ -1250,7 +1270,7 @@ template <class T> AttGradPlan att_grad_plan(int64_t heads, int64_t rows, int64_
     AttGradPlan p;
     p.blocks = cdiv(rows, kGradWaves * M);
     p.kblocks = cdiv(Lk, kGradWaves * M);
-    // both numbers of shares at once: the halves run side by side
+    // both numbers of shares at once: the halves run side by side (more than 64 gave nothing: 57 us, 60 us with up to 256, for 30 000 keys)
     const int64_t width = Dk > Dv ? Dk : Dv, tk = (Lk + kAttTile - 1) / kAttTile, tr = (rows + kAttTile - 1) / kAttTile;
     const double slots = (double)kAttCUs * att_resident(width), qn = (double)heads * p.blocks, kn = (double)heads * p.kblocks;
     double best = 0;
@@ -1322,7 +1342,8 @@ template <class T> int32_t attention_forward_impl(AttArgs<T>& p, void* scratch, 
     }
     DNH_LAUNCH_CHECK();
     if (p.splits > 1) {
-        hipLaunchKernelGGL((attention_join_kernel<Tile>), dim3(cdiv((int64_t)heads * p.rows, 4)), dim3(256), 0, s, p);
+        if (p.splits > 16) hipLaunchKernelGGL((attention_join_kernel<Tile, true>), dim3(heads * p.rows), dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((attention_join_kernel<Tile, false>), dim3(cdiv((int64_t)heads * p.rows, 4)), dim3(256), 0, s, p);
         DNH_LAUNCH_CHECK();
     }
     return DNH_OK;

@@ -395,3 +395,14 @@ def test_elements_whose_last_part_is_a_denormal(G, rng):
     out, _ = Tensor.crossAttention(*(G.ofNumpy(t) for t in (q, k, v)))
     err = np.abs(G.toNumpy(out).astype(np.float64) - v[:, :, :1])
     assert (err <= 2.0 ** -134 + 2 * 2.0 ** -24 * np.abs(v[:, :, :1])).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape", [(1, 3, 1, 1, 40000, 16, 100), (1, 1, 1, 40, 20000, 32, 32), (2, 1, 1, 7, 9001, 5, 3)])
+def test_long_sequences_in_many_shares(G, rng, dt, shape):
+    """More than 64 shares; some of them without a key."""
+    q, k, v, do = inputs(rng, dt, *shape)
+    mask = np.ones((shape[0], shape[4]), bool)
+    mask[0, 1000:7000] = False
+    mask[-1, 8000:] = rng.random(shape[4] - 8000) < 0.7
+    compare(G, q, k, v, do, mask, grads=False)
