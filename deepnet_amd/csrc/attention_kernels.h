@@ -1243,7 +1243,7 @@ template <class T> AttPlan att_plan(int64_t heads, int64_t rows, int64_t Lk, int
         p.blocks = cdiv(rows, (int64_t)p.waves * M);
         const double slots = (double)kAttCUs * att_resident(width) * 4 / p.waves;
         double best = 0;
-        for (int64_t n = 1; n <= kMaxShares && (n == 1 || 2 * n <= tiles + 1); n++) {
+        for (int64_t n = 1; n <= kMaxShares && (n == 1 || 2 * n <= tiles + 1); n += n < 16 ? 1 : n / 8) {
             const int64_t each = (tiles + n - 1) / n;
             const double bytes = n > 1 ? (double)heads * rows * n * width * sizeof(T) : 0.0;
             const double us = att_span_us((double)heads * p.blocks * n, att_walk_us<T>(width, 2, each), slots) + att_join_us(bytes);
