@@ -954,6 +954,22 @@ template <class A> __device__ __forceinline__ typename A::T att_lse(typename A::
     return lse == -(T)__builtin_inf() ? (T)__builtin_inf() : (T)(lse * (T)A::kBase);
 }
 
+// dS scales with what is upstream and may lie far below the numbers it is made of.  Cut in three parts it therefore carries a factor 2^64 until dq
+// and dk are stored: without it a part falls under bf16's least denormal, 2^-133, from dS = 2^-110 down.  Where that factor (or the rounding of a
+// first part) overflows, the sums are not finite, and the workgroup takes the float instructions.
+template <class Ops> constexpr typename Ops::T kAttUp = std::is_empty<typename Ops::Watch>::value ? 1 : 18446744073709551616.0;
+template <class Ops> __device__ __forceinline__ typename Ops::T att_ds(typename Ops::T prob, typename Ops::T dp_delta, typename Ops::T scale_up) {
+    return kAttUp<Ops> == 1 ? prob * dp_delta * scale_up : prob * scale_up * dp_delta;
+}
+template <class Ops> __device__ __forceinline__ bool att_finite(const typename Ops::Acc (&o)[Ops::ND]) {
+    typename Ops::T t = 0;
+#pragma unroll
+    for (int n = 0; n < Ops::ND; n++)
+#pragma unroll
+        for (int r = 0; r < Ops::Mma::R; r++) t += o[n][r] * typename Ops::T(0);
+    return t == typename Ops::T(0);
+}
+
 constexpr int kGradWaves = 4;
 template <class Ops> struct GradLds {
     typename Ops::Tile a[2], b[2];
@@ -981,6 +997,7 @@ __device__ __forceinline__ bool att_dq(const AttArgs<typename Ops::T>& p, GradLd
     Ops::load(g, p.d_out + att_row(p, p.sdo, b, hk, live ? row : 0), p.Dv, p.sdo.d, p.vec, h, watch);
     const T lse = live ? att_lse<A>(p.lse[att_row(p, p.slse, b, hk, row)]) : (T)__builtin_inf();
     const T delta = live ? p.delta[(size_t)head * p.rows + row] : T(0);
+    const T scale_up = p.scale * kAttUp<Ops>;
     Acc dq[ND];
 #pragma unroll
     for (int i = 0; i < ND; i++) dq[i] = 0;
@@ -1018,7 +1035,7 @@ __device__ __forceinline__ bool att_dq(const AttArgs<typename Ops::T>& p, GradLd
                 Acc s, dp;
                 Ops::scores(s, lds.a[buf], q, dp, lds.b[buf], g, u, c, h);
 #pragma unroll
-                for (int r = 0; r < A::R; r++) s[r] = A::exp_(s[r] * p.scale_base - lse) * (dp[r] - delta) * p.scale;
+                for (int r = 0; r < A::R; r++) s[r] = att_ds<Ops>(A::exp_(s[r] * p.scale_base - lse), dp[r] - delta, scale_up);
                 if (word != ~0u) {
 #pragma unroll
                     for (int r = 0; r < A::R; r++)
@@ -1029,7 +1046,7 @@ __device__ __forceinline__ bool att_dq(const AttArgs<typename Ops::T>& p, GradLd
             buf ^= 1;
         }
     }
-    if (!std::is_empty<typename Ops::Watch>::value && __syncthreads_or((int)Ops::failed(watch))) return false;
+    if (!std::is_empty<typename Ops::Watch>::value && __syncthreads_or((int)(Ops::failed(watch) || (live && !att_finite<Ops>(dq))))) return false;
     if (!live) return true;
     T* o;
     int64_t sd;
@@ -1040,7 +1057,7 @@ __device__ __forceinline__ bool att_dq(const AttArgs<typename Ops::T>& p, GradLd
         o = p.part_dq + (((size_t)split * p.B * p.Hk + head) * p.rows + row) * p.Dk;
         sd = 1;
     }
-    Ops::put(o, sd, p.Dk, dq, T(1), h);
+    Ops::put(o, sd, p.Dk, dq, T(1) / kAttUp<Ops>, h);
     return true;
 }
 
@@ -1074,6 +1091,7 @@ __device__ __forceinline__ bool att_dkv(const AttArgs<typename Ops::T>& p, GradL
     const int tiles = ((int)p.rows + kAttTile - 1) / kAttTile;
     const int t0 = split * p.ksplit_tiles, t1 = tiles < (int)(t0 + p.ksplit_tiles) ? tiles : (int)(t0 + p.ksplit_tiles);
     const bool any = __syncthreads_or((int)on);   // a block whose keys are all masked has nothing to add up
+    const T scale_up = p.scale * kAttUp<Ops>;
     typename Ops::Stage st;
     T lse = 0, delta = 0;                          // of row threadIdx.x of the tile in flight
     auto fetch = [&](int t) {
@@ -1108,14 +1126,14 @@ __device__ __forceinline__ bool att_dkv(const AttArgs<typename Ops::T>& p, GradL
             for (int r = 0; r < A::R; r++) {
                 const int i = u * M + A::acc_row(r, h);
                 const T pr = A::exp_(s[r] * p.scale_base - lds.lse[buf][i]);   // (a key that is off adds up something, too, which is dropped below)
-                dp[r] = pr * (dp[r] - lds.delta[buf][i]) * p.scale;
+                dp[r] = att_ds<Ops>(pr, dp[r] - lds.delta[buf][i], scale_up);
                 s[r] = pr;
             }
             Ops::outer(dv, lds.b[buf], s, dk, lds.a[buf], dp, u, c, h);
         }
         buf ^= 1;
     }
-    if (!std::is_empty<typename Ops::Watch>::value && __syncthreads_or((int)Ops::failed(watch))) return false;
+    if (!std::is_empty<typename Ops::Watch>::value && __syncthreads_or((int)(Ops::failed(watch) || (on && !(att_finite<Ops>(dk) && att_finite<Ops>(dv)))))) return false;
     if (!in) return true;
     T *ok, *ov;
     int64_t sk, sv;
@@ -1134,7 +1152,7 @@ __device__ __forceinline__ bool att_dkv(const AttArgs<typename Ops::T>& p, GradL
 #pragma unroll
         for (int i = 0; i < ND; i++) dk[i] = dv[i] = 0;
     }
-    Ops::put(ok, sk, p.Dk, dk, T(1), h);
+    Ops::put(ok, sk, p.Dk, dk, T(1) / kAttUp<Ops>, h);
     Ops::put(ov, sv, p.Dv, dv, T(1), h);
     return true;
 }
