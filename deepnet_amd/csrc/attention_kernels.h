@@ -377,8 +377,9 @@ template <class A, int DP, int WAVES = 4, bool WHOLE = true> struct AttOps {
 // v_mfma_f32_32x32x16_bf16 does in 32 cycles what v_mfma_f32_32x32x2_f32 does in 512.  A float is the exact sum of three bf16 numbers (each
 // the remainder so far, rounded to nearest: 8 + 8 + 8 significant bits), every product of two parts is exact in the instruction, and of the nine
 // partial products the six largest are kept: those dropped are below 2^-23 |a b| together (2 u of one rounded product), and 6 x 32 cycles take
-// the place of 512.  Parts of elements below 2^-109 fall under bf16's smallest denormal: such an element is kept to 2^-134.  An element of
-// 2^127 or more (infinities, NaN) has no such parts: the workgroup that meets one starts again on the float instructions.
+// the place of 512.  The last part of an element below 2^-109 falls under bf16's smallest denormal: a workgroup that meets one (zero
+// apart) starts again on the float instructions.  So does one whose sums are not finite: an element that rounds to an infinity in 8 bits, and an
+// infinite one, has NaN as its last part.  Probabilities, which float exponentials flush at 2^-126, are kept to 2^-134; dS is scaled (kAttUp).
 //
 // The instruction's K = 16: lane l supplies A[l % 32][8 (l / 32) + i] and B[8 (l / 32) + i][l % 32], i = 0 .. 7.  Its result lies as that of
 // v_mfma_f32_32x32x2_f32, so registers 8 j .. 8 j + 7 of lane half h are the rows 16 j + 4 h + { 0 .. 3, 8 .. 11 }: with K numbered in this order
@@ -409,11 +410,16 @@ template <int DP, int WAVES, bool PIN> struct AttOpsX3 {
     typedef uint32_t U2 __attribute__((ext_vector_type(2)));
     typedef uint32_t U4 __attribute__((ext_vector_type(4)));
     typedef uint16_t H2 __attribute__((ext_vector_type(2)));
-    struct Watch {                                     // the largest first parts, without their signs
-        H2 top = 0;
-        __device__ __forceinline__ void see(uint32_t hi) { top = __builtin_elementwise_max(top, __builtin_bit_cast(H2, hi & 0x7FFF7FFFu)); }
+    struct Watch {                                     // the least first part that is not zero: -2 times it, which loses its sign, is the largest
+        H2 least = 0;
+        __device__ __forceinline__ void see(uint32_t hi) {
+            H2 x;
+            asm("v_pk_mul_lo_u16 %0, %1, %2" : "=v"(x) : "v"(hi), "s"(0xFFFEFFFEu));   // (the compiler makes a shift and a subtraction of it)
+            least = __builtin_elementwise_max(least, x);
+        }
     };
-    static __device__ __forceinline__ bool failed(const Watch& w) { return w.top[0] >= 0x7F00 || w.top[1] >= 0x7F00; }   // 2^127
+    // 2^-109 (a first part that was rounded up to it comes from 2^-109 (1 - 2^-9), which has parts, too)
+    static __device__ __forceinline__ bool failed(const Watch& w) { return w.least[0] > 0x10000 - 2 * 0x0900 || w.least[1] > 0x10000 - 2 * 0x0900; }
     struct __attribute__((aligned(16))) Tile {
         uint16_t x[3 * PLANE];
     };
@@ -647,6 +653,16 @@ template <class A> __device__ __forceinline__ typename A::T att_lse_of(typename 
     return l == T(0) ? -(T)__builtin_inf() : (T)((m + A::log_(l)) * (T)(1.0 / A::kBase));
 }
 
+// whether none of a lane's sums is infinite or NaN
+template <class Ops> __device__ __forceinline__ bool att_finite(const typename Ops::Acc (&o)[Ops::ND]) {
+    typename Ops::T t = 0;
+#pragma unroll
+    for (int n = 0; n < Ops::ND; n++)
+#pragma unroll
+        for (int r = 0; r < Ops::Mma::R; r++) t += o[n][r] * typename Ops::T(0);
+    return t == typename Ops::T(0);
+}
+
 // Stores a wavefront's result out^T (lane: row, registers: width) or its share of it.
 template <class Ops>
 __device__ __forceinline__ void att_store(const AttArgs<typename Ops::T>& p, const typename Ops::Acc (&o)[Ops::ND], uint32_t head, int b, int hk, uint32_t row,
@@ -748,7 +764,7 @@ __device__ __forceinline__ bool att_forward(const AttArgs<typename Ops::T>& p, A
             buf ^= 1;
         }
     }
-    if (!std::is_empty<typename Ops::Watch>::value && __syncthreads_or((int)Ops::failed(watch))) return false;
+    if (!std::is_empty<typename Ops::Watch>::value && __syncthreads_or((int)(Ops::failed(watch) || (live && !(att_finite<Ops>(o) && l * T(0) == T(0)))))) return false;
     l = across_sum<A>(l);
     if (live) att_store<Ops>(p, o, head, b, hk, row, split, h, m, l);
     return true;
@@ -955,21 +971,12 @@ template <class A> __device__ __forceinline__ typename A::T att_lse(typename A::
 }
 
 // dS scales with what is upstream and may lie far below the numbers it is made of.  Cut in three parts it therefore carries a factor 2^64 until dq
-// and dk are stored: without it a part falls under bf16's least denormal, 2^-133, from dS = 2^-110 down.  Where that factor (or the rounding of a
-// first part) overflows, the sums are not finite, and the workgroup takes the float instructions.
+// and dk are stored: without it a part falls under bf16's least denormal, 2^-133, from dS = 2^-110 down.  Where that factor overflows, the
+// sums are not finite.
 template <class Ops> constexpr typename Ops::T kAttUp = std::is_empty<typename Ops::Watch>::value ? 1 : 18446744073709551616.0;
 template <class Ops> __device__ __forceinline__ typename Ops::T att_ds(typename Ops::T prob, typename Ops::T dp_delta, typename Ops::T scale_up) {
     return kAttUp<Ops> == 1 ? prob * dp_delta * scale_up : prob * scale_up * dp_delta;
 }
-template <class Ops> __device__ __forceinline__ bool att_finite(const typename Ops::Acc (&o)[Ops::ND]) {
-    typename Ops::T t = 0;
-#pragma unroll
-    for (int n = 0; n < Ops::ND; n++)
-#pragma unroll
-        for (int r = 0; r < Ops::Mma::R; r++) t += o[n][r] * typename Ops::T(0);
-    return t == typename Ops::T(0);
-}
-
 constexpr int kGradWaves = 4;
 template <class Ops> struct GradLds {
     typename Ops::Tile a[2], b[2];

@@ -375,8 +375,9 @@ int32_t dnh_token_log_probs_grad(const DnhTensor* d_logits, const DnhTensor* log
  * head h reads key head h / (Hq / Hk).  mask [B; Lk] (bool) or NULL: keys with false are not attended to, and what k and v hold there
  * (infinities and NaN included) is not used.  A sequence without keys has out 0 and lse -inf.  scale defaults to 1 / sqrt(Dk).
  * Widths up to 128.  [B; L; H; D] tensors are passed as permuted views.  Single precision: where widths are multiples of 4 along contiguous
- * axes the products are taken on the bf16 matrix instructions from three parts of every number, with the error of a float product; elements
- * below 2^-109 are kept to 2^-134 there, elements of 2^127 and more (and infinities) take the float instructions. */
+ * axes the products are taken on the bf16 matrix instructions from three parts of every number, with the error of a float product; a
+ * workgroup that meets an element below 2^-109 (zero apart), or whose sums are not finite, takes the float instructions.  Before they are divided by
+ * their denominator, sums over the keys of e^(score - largest score) |v| must stay in the type's range. */
 int32_t dnh_cross_attention(const DnhTensor* out, const DnhTensor* lse, const DnhTensor* q, const DnhTensor* k, const DnhTensor* v,
                             const DnhTensor* mask_bool, const void* scale, void* scratch, size_t scratch_bytes, void* stream);
 /* Gradients of sum(d_out out) with out and lse as dnh_cross_attention gave them: d_q like q, d_k like k, d_v like v, those of a shared key

@@ -14,8 +14,9 @@ pytestmark = pytest.mark.gpu
 F32 = np.float32
 
 
-def grad_bounds(o, do, out, lse):
-    """d_q, d_k, d_v and their bounds, for an oracle whose scores leave every key a probability above 2^-60."""
+def grad_bounds(o, do, out, lse, least=0.0, part=6 * 2.0 ** -126):
+    """d_q, d_k, d_v and their bounds, for an oracle whose scores leave every key a probability above 2^-60.  part: what may vanish of a
+    product of d_out and v; least: the same of one of dS and of each of the three roundings that make dS."""
     do, out, lse, u = do.astype(np.float64), out.astype(np.float64), lse.astype(np.float64)[..., None], o.u
     T = lambda a: a.transpose(0, 1, 3, 2)
     p = np.exp(o.s - lse)
@@ -25,11 +26,11 @@ def grad_bounds(o, do, out, lse):
     ds = p * (dp - delta) * o.scale
     n, rows = do.shape[-1], do.shape[2]
     rp = o.r[..., None] + 4 * u * np.abs(lse)
-    e = np.abs(ds) * (rp + 8 * u) + abs(o.scale) * p * ((n + 2) * u * (dpa + da) + 6 * n * 2.0 ** -126)
+    e = np.abs(ds) * (rp + 8 * u) + abs(o.scale) * p * ((n + 2) * u * (dpa + da) + n * part) + 3 * least
     tiny = 2.0 ** -149
-    return [(ds @ o.k, (e + (o.lk + 4) * u * np.abs(ds)) @ np.abs(o.k) + tiny),
-            (T(ds) @ o.q, T(e + (rows + 4) * u * np.abs(ds)) @ np.abs(o.q) + tiny),
-            (T(p) @ do, T(p * (rp + (rows + 4) * u)) @ np.abs(do) + rows * 6 * 2.0 ** -126)]
+    return [(ds @ o.k, (e + (o.lk + 4) * u * np.abs(ds)) @ np.abs(o.k) + o.lk * least + tiny),
+            (T(ds) @ o.q, T(e + (rows + 4) * u * np.abs(ds)) @ np.abs(o.q) + rows * least + tiny),
+            (T(p) @ do, T(p * (rp + (rows + 4) * u)) @ np.abs(do) + rows * part)]
 
 
 def check(G, q, k, v, do, scale):
@@ -88,3 +89,29 @@ def test_an_infinity_upstream_reaches_its_own_row_only(G, rng):
     bad[7] = True
     assert not np.isfinite(dq[0, 0, bad]).any() and np.isfinite(dq[0, 0, ~bad]).all()
     assert (dv[0, 0, :, 3] == np.inf).all() and np.isfinite(np.delete(dv[0, 0], 3, 1)).all()
+
+
+@pytest.mark.parametrize("Lq, D", [(70, 64), (40, 128), (33, 32), (20, 64), (70, 62)])
+@pytest.mark.parametrize("which", "q k v do".split())
+def test_elements_of_which_bf16_parts_hold_half(G, rng, Lq, D, which):
+    """One operand around 2^-122, where three bf16 parts keep 12 bits; the others and the scale bring the scores to about 1 and dS to where a float
+    holds it.  The float instructions keep denormals: a sum of n products is besides off by n 2^-149, dS by three such roundings."""
+    t = dict(zip(("q", "k", "v", "do"), inputs(rng, F32, 1, 2, 2, Lq, 12, D, D)))
+    n = t[which].shape
+    t[which] = (np.where(rng.random(n) < 0.5, -1, 1) * (1 + rng.random(n)) * 2.0 ** -122).astype(F32)
+    scale = 4.0
+    if which in "qk":
+        other = "k" if which == "q" else "q"
+        t[other], t["do"], scale = t[other] * F32(2.0 ** 60), t["do"] * F32(2.0 ** -56), 2.0 ** 58
+    else:
+        t["q"] *= F32(2.0 ** -20)
+    q, k, v, do = (t[x] for x in ("q", "k", "v", "do"))
+    o = Oracle(q, k, v, None, scale, unit(F32))
+    out, lse = Tensor.crossAttention(*(G.ofNumpy(x) for x in (q, k, v)), scale=scale)
+    within(G.toNumpy(out), o.out, (o.p * (2 * o.r + 28 * o.u)[..., None]) @ np.abs(o.v) + 12 * 2.0 ** -149, "out")
+    within(G.toNumpy(lse), o.lse, o.lse_bound(), "lse")
+    on, ln = o.out.astype(F32), o.lse.astype(F32)
+    got = Tensor.crossAttentionGrad(*(G.ofNumpy(x) for x in (do, q, k, v, on, ln)), scale=scale)
+    for g, (ref, bound), what in zip(got, grad_bounds(o, do, on, ln, 2.0 ** -149, 2.0 ** -149), ("d_q", "d_k", "d_v")):
+        within(G.toNumpy(g), ref, bound, what)
+
