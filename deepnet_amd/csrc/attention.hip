@@ -91,6 +91,7 @@ AttArgs<T> common_args(const DnhTensor* q, const DnhTensor* k, const DnhTensor* 
     p.scale_base = (T)((double)p.scale * MmaOf<T>::Tile::kBase);
     p.vec = p.sq.d == 1 && p.sk.d == 1 && p.sv.d == 1;
     p.whole = p.vec && p.Dk % kVecN<T> == 0 && p.Dv % kVecN<T> == 0;
+    p.exact = option(OPT_ATTENTION_BF16X3) == 0;
     // with 2^(l - 1) < Lq <= 2^l and mul = ceil(2^(31 + l) / Lq): mul Lq exceeds 2^(31 + l) by less than 2^l, so r mul 2^-(31 + l) exceeds
     // r / Lq by less than r 2^-31 / Lq < 1 / Lq, and the integer parts agree
     int l = 0;

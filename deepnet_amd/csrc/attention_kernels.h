@@ -80,6 +80,7 @@ template <class T> struct AttArgs {
     T scale, scale_base;      // scale, and scale x log e in the exponentials' base
     bool vec;                 // q, k, v (and d_out) are contiguous along their last axis
     bool whole;               // and their widths are whole 16-byte pieces
+    bool exact;               // no bf16 parts
     // workgroups of a key head: row blocks x shares of the keys (forward, dq), key blocks x shares of the rows (dk, dv)
     uint32_t blocks, splits, split_tiles;
     uint32_t kblocks, ksplits, ksplit_tiles;
@@ -778,7 +779,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel
         AttLds<Exact> exact;
     } lds;
     if constexpr (!std::is_same<First, Exact>::value)
-        if (att_forward<First, WAVES>(p, lds.first)) return;
+        if (!p.exact && att_forward<First, WAVES>(p, lds.first)) return;
     att_forward<Exact, WAVES>(p, lds.exact);
 }
 
@@ -1181,11 +1182,11 @@ __global__ __launch_bounds__(64 * kGradWaves, DP <= 64 ? 2 : 1) void attention_g
     const uint32_t at = front ? blockIdx.x : blockIdx.x - first;
     if (front == dq_first) {
         if constexpr (!std::is_same<First, Exact>::value)
-            if (att_dq(p, lds.first, at)) return;
+            if (!p.exact && att_dq(p, lds.first, at)) return;
         att_dq(p, lds.exact, at);
     } else {
         if constexpr (!std::is_same<First, Exact>::value)
-            if (att_dkv(p, lds.first, at)) return;
+            if (!p.exact && att_dkv(p, lds.first, at)) return;
         att_dkv(p, lds.exact, at);
     }
 }

@@ -96,6 +96,7 @@ enum Option {
     OPT_COUNT_ONE_LAUNCH,    // 1: countTrue of a whole contiguous mask in one launch (arrival counters); 0: the general two-pass fold
     OPT_LOOKBACK_SPINS,      // polls a one-pass compaction's tile spends on predecessors that have not published before it counts for itself
     OPT_INVERT_TOURNAMENT,   // -1: matrices of more than 32 rows pick a panel's pivots by tournament; 0: never; 1: always
+    OPT_ATTENTION_BF16X3,    // 1: single-precision attention on the bf16 matrix instructions where its layout allows; 0: float instructions
     OPT_COUNT
 };
 int option(Option o);

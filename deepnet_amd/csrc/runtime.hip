@@ -149,6 +149,7 @@ constexpr OptionDef kOptions[OPT_COUNT] = {
     {"count_one_launch", 1, 0, 1},
     {"lookback_spins", 1 << 18, 0, 1 << 30},
     {"invert_tournament", -1, -1, 1},
+    {"attention_bf16x3", 1, 0, 1},
 };
 std::atomic<int> g_options[OPT_COUNT];
 std::once_flag g_options_once;

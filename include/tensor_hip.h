@@ -172,6 +172,8 @@ int32_t dnh_last_error(char* buf, size_t n);
  *                       updates the columns the next panel does not need on a stream of the library's own, beside that panel's
  *                       tournament; 0: every size eliminates its panels column by column with partial pivoting in one
  *                       workgroup; 1: tournament for every size
+ *   "attention_bf16x3"  1 (default): single-precision attention on the bf16 matrix instruction, three parts per float, where widths are
+ *                       multiples of 4 along contiguous axes; 0: float instructions (which up to 32 rows of a key head take in any case)
  * Unknown names and values outside an option's range: DNH_ERR_INVALID_ARG. */
 int32_t dnh_set_option(const char* name, int32_t value);
 int32_t dnh_get_option(const char* name, int32_t* value);
@@ -376,7 +378,8 @@ int32_t dnh_token_log_probs_grad(const DnhTensor* d_logits, const DnhTensor* log
  * (infinities and NaN included) is not used.  A sequence without keys has out 0 and lse -inf.  scale defaults to 1 / sqrt(Dk).
  * Widths up to 128.  [B; L; H; D] tensors are passed as permuted views.  Single precision: where widths are multiples of 4 along contiguous
  * axes the products are taken on the bf16 matrix instructions from three parts of every number, with the error of a float product; a
- * workgroup that meets an element below 2^-109 (zero apart), or whose sums are not finite, takes the float instructions.  Before they are divided by
+ * workgroup that meets an element below 2^-109 (zero apart), or whose sums are not finite, takes the float instructions, as all do with the option
+ * "attention_bf16x3" = 0.  Before they are divided by
  * their denominator, sums over the keys of e^(score - largest score) |v| must stay in the type's range. */
 int32_t dnh_cross_attention(const DnhTensor* out, const DnhTensor* lse, const DnhTensor* q, const DnhTensor* k, const DnhTensor* v,
                             const DnhTensor* mask_bool, const void* scale, void* scratch, size_t scratch_bytes, void* stream);

@@ -6,6 +6,7 @@ below 2^-126 is lost of it, and results round at the least denormal, 2^-149."""
 import numpy as np
 import pytest
 
+from deepnet_amd import native
 from deepnet_amd.tensor import Tensor
 
 from test_gpu_model_attention import Oracle, inputs, unit, within
@@ -115,3 +116,24 @@ def test_elements_of_which_bf16_parts_hold_half(G, rng, Lq, D, which):
     for g, (ref, bound), what in zip(got, grad_bounds(o, do, on, ln, 2.0 ** -149, 2.0 ** -149), ("d_q", "d_k", "d_v")):
         within(G.toNumpy(g), ref, bound, what)
 
+
+
+@pytest.mark.parametrize("Lq, Lk, D", WIDTHS)
+def test_the_float_instructions_by_option(G, rng, Lq, Lk, D):
+    """attention_bf16x3 = 0: the same bounds, and for layouts that would take the parts other bits (sums rounded at other places)."""
+    q, k, v, do = inputs(rng, F32, 1, 2, 2, Lq, Lk, D, D)
+    scale = float(F32(1 / np.sqrt(D)))
+    o = Oracle(q, k, v, None, scale, unit(F32))
+    results = []
+    for parts in (1, 0):
+        with native.option("attention_bf16x3", parts):
+            out, lse = (G.toNumpy(t) for t in Tensor.crossAttention(*(G.ofNumpy(t) for t in (q, k, v)), scale=scale))
+            within(out, o.out, o.out_bound(), "out")
+            within(lse, o.lse, o.lse_bound(), "lse")
+            on, ln = o.out.astype(F32), o.lse.astype(F32)
+            got = [G.toNumpy(t) for t in Tensor.crossAttentionGrad(*(G.ofNumpy(t) for t in (do, q, k, v, on, ln)), scale=scale)]
+            for g, (ref, bound), what in zip(got, o.grad(do, on, ln), ("d_q", "d_k", "d_v")):
+                within(g, ref, bound, what)
+            results.append([out, *got])
+    for a, b in zip(*results):
+        assert np.array_equal(a, b) == (D % 4 != 0)
