@@ -72,7 +72,7 @@ template <class X> __device__ __forceinline__ X from_lane_below(X x) {       // 
     return x;
 }
 
-// Where a wavefront spreads some lanes' elements over all lanes (LDS accesses of one wavefront are served in order).
+// Where a wavefront spreads some lanes' elements over all lanes.
 template <class T> struct Spread {
     T x[64];
     uint32_t first[64], taken[64];
@@ -179,8 +179,12 @@ template <class T> struct TopList {
                 sp.first[rank] = first;
                 sp.taken[rank] = taken;
             }
+            wave_lds_fence();
             const uint32_t j = sp.first[lane / C] + step(lane % C);
-            offer(sp.x[lane], j, lane / C < __popcll(m) && j < end && j != sp.taken[lane / C], K);
+            const T v_lane = sp.x[lane];
+            const uint32_t taken_lane = sp.taken[lane / C];
+            wave_lds_fence();                            // (the next lanes' elements go to the same places)
+            offer(v_lane, j, lane / C < __popcll(m) && j < end && j != taken_lane, K);
 #pragma unroll
             for (int k = 0; k < L; k++) m &= m - 1;      // (0 stays 0)
             m &= __ballot(big >= floor_v);

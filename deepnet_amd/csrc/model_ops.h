@@ -111,6 +111,14 @@ inline int32_t get_scratch(hipStream_t stream, size_t need, void* given, size_t 
     return workspace(stream, need, out, lease);
 }
 
+// Between LDS accesses of one wavefront whose lanes hand each other data: the hardware serves them in order, and this keeps the compiler from
+// moving them across or from using again what a lane has read before.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 inline size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 // Threads of a 256-thread workgroup that share a row of `items` accesses: a power of two of 4..256.
