@@ -236,7 +236,7 @@ template <class T> __device__ __forceinline__ void take(T x, T m, double& s, dou
     s += (double)e;
     a += (double)(e * entropy_factor(d));
 }
-// the larger one; of a number and a NaN the number
+// the larger one; of a number and a quiet NaN the number (the instruction makes a NaN of a number and a signaling one)
 __device__ __forceinline__ float larger(float x, float y) {
     float r;
     // (fmaxf first quiets both operands: three instructions.  The operands must not come straight from a transcendental instruction, whose
@@ -339,11 +339,11 @@ __global__ __launch_bounds__(kBlock, TOP ? 5 : 1) void log_probs_kernel(LogProbA
                 }
             }
         }
-        T big = v[0][0];
+        T big = neg_inf<T>();                                                       // of the numbers; NaN of either kind is passed over
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int e = 0; e < N; e++) big = larger(big, v[u][e]);
+            for (int e = 0; e < N; e++) big = v[u][e] > big ? v[u][e] : big;
         if (__ballot(big > m)) {
             T to = big > m ? big : m;
 #pragma unroll

@@ -41,3 +41,22 @@ def test_a_few_lanes_better_in_every_step(G, rng, dt, lanes, rows, vocab):
         np.testing.assert_array_equal(alternatives(G, X, K), want[:, :K])
     down = G.ofNumpy(np.ascontiguousarray(x[:520, :9000].T)).T     # the vocabulary along a strided axis
     np.testing.assert_array_equal(alternatives(G, down, 8), best(x[:520, :9000], 8))
+
+
+@pytest.mark.parametrize("dt, nan", [(np.float32, 0x7FC00000), (np.float32, 0x7FA00001), (np.float32, 0xFF800001),
+                                     (np.float64, 0x7FF8000000000000), (np.float64, 0x7FF4000000000001), (np.float64, 0xFFF0000000000001)])
+@pytest.mark.parametrize("rows,vocab", [(4, 30000), (600, 9001)])
+def test_no_kind_of_nan_hides_the_numbers_beside_it(G, rng, dt, nan, rows, vocab):
+    """Quiet and signaling NaNs right behind and far behind the best element, in its lane: the alternatives are those of the numbers."""
+    x = rng.standard_normal((rows, vocab)).astype(dt)
+    bits = x.view(np.uint32 if dt == np.float32 else np.uint64)
+    at = rng.integers(vocab - 3000, vocab - 2000, rows)
+    for r in range(rows):
+        x[r, at[r]] = 50
+        bits[r, at[r] + 1:at[r] + 4] = nan
+        bits[r, at[r] + 1024] = nan
+    tok = np.zeros(rows, np.int64)
+    lp, lse, ent, tv, ti = (G.toNumpy(t) for t in Tensor.tokenLogProbs(G.ofNumpy(x), G.ofNumpy(tok), 5))
+    np.testing.assert_array_equal(ti, best(x, 5))
+    for t in (lp, lse, ent, tv):
+        assert np.isnan(t).all()
