@@ -928,7 +928,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs<typename A:
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
-    __builtin_amdgcn_wave_barrier();                  // (a wavefront uses its own weights only)
+    wave_lds_fence();                                 // (a wavefront uses its own weights only)
     const T f = l == T(0) ? T(0) : T(1) / l;
     T* orow = p.o + att_row(p, p.so, b, hk, r);
     const T* part = p.part_o + row * p.splits * p.Dv;
