@@ -23,9 +23,15 @@ int g_device = 0;
 std::mutex g_pinned_mu;
 std::map<uintptr_t, size_t> g_pinned;   // blocks handed out by dnh_host_alloc
 int g_cus = 256;
-std::map<hipStream_t, int32_t*> g_error_flags;   // one index-error word per stream, so concurrent streams do not see each other's errors
+// One index-error word per stream, so concurrent streams do not see each other's errors.
+struct ErrorWord {
+    int32_t* p = nullptr;
+    bool in_graph = false;   // handed out while the stream was being captured: a graph may write to it as long as it lives
+};
+std::map<hipStream_t, ErrorWord> g_error_flags;
 // Words for g_error_flags, allocated and cleared once when the device is chosen: the first indexing call of a stream may be one that is
-// being captured into a graph, where nothing can be allocated.  A word goes back when its stream is destroyed.
+// being captured into a graph, where nothing can be allocated.  A word goes back when its stream is destroyed, unless a
+// graph has it: another stream would then report that graph's errors.
 std::vector<int32_t*> g_spare_flags;
 constexpr int kSpareFlags = 1024;
 
@@ -182,18 +188,21 @@ int option(Option o) {
     return g_options[o].load(std::memory_order_relaxed);
 }
 int32_t error_flag_ptr(hipStream_t stream, int32_t** out) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (stream) DNH_HIP(hipStreamIsCapturing(stream, &st));   // (the default stream cannot be captured)
     std::lock_guard<std::mutex> lock(g_mu);
-    int32_t*& p = g_error_flags[stream];
-    if (!p) {
+    ErrorWord& w = g_error_flags[stream];
+    if (!w.p) {
         if (!g_spare_flags.empty()) {
-            p = g_spare_flags.back();
+            w.p = g_spare_flags.back();
             g_spare_flags.pop_back();
         } else {
-            DNH_TRY(device_malloc((void**)&p, sizeof(int32_t), "index error word"));
-            DNH_HIP(hipMemset(p, 0, sizeof(int32_t)));
+            DNH_TRY(device_malloc((void**)&w.p, sizeof(int32_t), "index error word"));
+            DNH_HIP(hipMemset(w.p, 0, sizeof(int32_t)));
         }
     }
-    *out = p;
+    if (st != hipStreamCaptureStatusNone) w.in_graph = true;
+    *out = w.p;
     return DNH_OK;
 }
 
@@ -271,8 +280,9 @@ static void drop_workspace(hipStream_t stream) {
     std::lock_guard<std::mutex> lock(g_mu);
     auto ef = g_error_flags.find(stream);
     if (ef != g_error_flags.end()) {
-        // (the stream has been synchronised: nothing that could set the word is left)
-        if (ef->second && hipMemset(ef->second, 0, sizeof(int32_t)) == hipSuccess) g_spare_flags.push_back(ef->second);
+        // (the stream has been synchronised: nothing but a graph could still set the word)
+        int32_t* p = ef->second.p;
+        if (p && !ef->second.in_graph && hipMemset(p, 0, sizeof(int32_t)) == hipSuccess) g_spare_flags.push_back(p);
         g_error_flags.erase(ef);
     }
     auto it = g_ws.find(stream);

@@ -179,6 +179,8 @@ int32_t dnh_set_option(const char* name, int32_t value);
 int32_t dnh_get_option(const char* name, int32_t* value);
 /* Reads and clears the device-side index error flag set by gather/scatter kernels on `stream`
  * (synchronises the stream; every stream has its own flag, so concurrent streams do not see each other's errors).  *code = DNH_OK or DNH_ERR_INDEX_OUT_OF_RANGE.
+ * A call that was captured into a graph sets the flag of the stream it was captured on, wherever the graph is replayed: wait for the replay, then ask that
+ * stream.  Once that stream is destroyed nobody is told (the flag is not given to another stream).
  * Replaces the error word + `Cfg.Stacktrace` read-back of Cuda/CudaKernels.fs:323-342, 385-398. */
 int32_t dnh_async_error(void* stream, int32_t* code);
 
