@@ -483,6 +483,7 @@ __global__ __launch_bounds__(kJoinThreads) void embedding_join_kernel(GradTarget
 // clear) 40 us against 47; 500 tokens into 500 rows of 2000, where the sums are most of it, 12.4 us against 14.3.
 constexpr uint32_t kFewTokens = 512;
 constexpr int kFillRows = 2048;   // most rows of a block that is cleared at once
+constexpr size_t kFewScratch = 256;   // what the query answers for them: none of it is used, but a call with less than the query says is refused
 bool few_tokens(int64_t n, int64_t width) { return n <= kFewTokens && n * width <= (1 << 28); }   // (a grid of fewer than 2^32 threads for any width)
 template <class T, bool VEC>
 __global__ __launch_bounds__(kBlock) void embedding_grad_few_kernel(GradTarget<T> tg, TokenSource src, const T* __restrict__ g, RowPlan<1> gp, int64_t gd, uint32_t chunks,
@@ -622,6 +623,11 @@ GradPlan grad_plan(uint32_t n, int64_t vocab, int64_t width) {
     p.nchunks = cdiv(n, p.chunk);
     p.pitch = (width + 1) / 2 * 2;
     const bool small = n <= kSmallSort;
+    if (few_tokens(n, width)) {
+        p.list_bytes = p.counts_bytes = p.partial_bytes = 0;
+        p.total = n ? kFewScratch : 0;
+        return p;
+    }
     p.list_bytes = up256((size_t)n * 4);
     p.counts_bytes = small ? 0 : up256((size_t)kMaxDigits * p.nchunks * 4);
     p.partial_bytes = up256((size_t)p.pieces * 2 * (size_t)p.pitch * 8);
@@ -641,11 +647,11 @@ int32_t embedding_grad(const DnhTensor* dt, const DnhTensor* tokens, const DnhTe
     char* ws = nullptr;
     WorkspaceLease lease;
     DNH_TRY(error_flag_ptr(s, &src.err));
-    // (few tokens use none of it; the call's contract, above all what a captured call has to bring, is the same at every size)
-    DNH_TRY(get_scratch(s, n ? p.total : 0, scratch, scratch_bytes, (void**)&ws, lease, "dnh_embedding_grad"));
+    const bool few = few_tokens(n, width);
+    if (!few || scratch) DNH_TRY(get_scratch(s, n ? p.total : 0, scratch, scratch_bytes, (void**)&ws, lease, "dnh_embedding_grad"));
     const RowPlan<1> gp = make_row_plan<1>(nd, {d_out});
     const bool vec = d_out->stride[nd] == 1;
-    if (few_tokens(n, width)) {
+    if (few) {
         const unsigned chunks = cdiv(width, 64 * (vec ? kVecN<T> : 1));
         // blocks of 16 to 32 KB, a workgroup each until there are eight per compute unit
         uint32_t block_rows = 1;

@@ -350,7 +350,8 @@ int32_t dnh_embedding(const DnhTensor* t, const DnhTensor* table, const DnhTenso
 /* d_table[v, :] = scale * sum of d_out[i, :] over the i with tokens[i] = v, for every row v (accumulate = 0: rows of absent tokens
  * become zero), or that sum added to d_table (accumulate = 1: rows of absent tokens stay untouched).  Each row's
  * addends are summed in double precision, in an order that depends on the tokens alone; one rounding at the end.  A token outside
- * the table sets the stream's error flag and contributes nothing.  Up to 2^27 tokens. */
+ * the table sets the stream's error flag and contributes nothing.  Up to 2^27 tokens.  Up to 512 tokens (and 2^28 elements of d_out) use no scratch
+ * memory, captured or not; the query then answers 256 bytes, which a call that is given less is refused for all the same. */
 int32_t dnh_embedding_grad(const DnhTensor* d_table, const DnhTensor* tokens_i64, const DnhTensor* d_out, const void* scale, int32_t accumulate,
                            void* scratch, size_t scratch_bytes, void* stream);
 int32_t dnh_embedding_grad_scratch_bytes(int64_t tokens, int64_t vocab, int64_t width, size_t* bytes);

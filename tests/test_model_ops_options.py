@@ -1,4 +1,5 @@
-"""CPU: the switch of the language-model operators."""
+"""CPU: the switch of the language-model operators, and scratch memory that they do not need."""
+import ctypes as C
 import os
 
 import pytest
@@ -17,3 +18,15 @@ def test_attention_option():
     for bad in (-1, 2):
         with pytest.raises(ValueError):
             native.set_option("attention_bf16x3", bad)
+
+
+def test_few_tokens_ask_for_next_to_no_scratch_memory():
+    """The gradient of up to 512 tokens keeps nothing between launches, however wide the rows are."""
+    lib, n = native.load(), C.c_size_t()
+    for tokens, width in ((1, 1), (512, 1 << 19), (512, 300), (7, 1 << 23)):
+        native.check(lib.dnh_embedding_grad_scratch_bytes(tokens, 50000, width, C.byref(n)))
+        assert n.value <= 256, (tokens, width, n.value)
+    native.check(lib.dnh_embedding_grad_scratch_bytes(513, 50000, 300, C.byref(n)))
+    assert n.value > 513 * 8
+    native.check(lib.dnh_embedding_grad_scratch_bytes(512, 50000, 1 << 20, C.byref(n)))       # too much for one launch
+    assert n.value > 64 * 2 * (1 << 20) * 8
