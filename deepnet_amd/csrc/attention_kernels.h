@@ -1360,9 +1360,14 @@ template <class T> int32_t attention_forward_impl(AttArgs<T>& p, void* scratch, 
         else hipLaunchKernelGGL((attention_few_kernel<Few, 128, false>), grid, dim3(64), 0, s, p);
     } else {
         att_widths<T>(width, [&](auto dp) {
-            if (pl.waves == 2 && p.whole) hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 2, true>), grid, dim3(128), 0, s, p);
-            else if (pl.waves == 2) hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 2, false>), grid, dim3(128), 0, s, p);
-            else if (p.whole) hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 4, true>), grid, dim3(256), 0, s, p);
+            if constexpr (2 * Tile::M > kFewRows) {   // (else two wavefronts have no more rows than the kernel for few takes)
+                if (pl.waves == 2) {
+                    if (p.whole) hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 2, true>), grid, dim3(128), 0, s, p);
+                    else hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 2, false>), grid, dim3(128), 0, s, p);
+                    return;
+                }
+            }
+            if (p.whole) hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 4, true>), grid, dim3(256), 0, s, p);
             else hipLaunchKernelGGL((attention_kernel<Tile, dp.value, 4, false>), grid, dim3(256), 0, s, p);
         });
     }

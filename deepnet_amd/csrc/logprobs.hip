@@ -203,7 +203,6 @@ template <class T> struct LogProbArgs {
     int64_t* top_i;
     int64_t top_vd, top_id;
     int K;
-    uint32_t rows;
     int32_t* err;
 };
 
@@ -474,7 +473,6 @@ int32_t log_probs(const DnhTensor* log_probs, const DnhTensor* lse, const DnhTen
     p.top_vd = top_v ? top_v->stride[nd] : 0;
     p.top_id = top_i ? top_i->stride[nd] : 0;
     p.K = K;
-    p.rows = rows;
     p.err = nullptr;
     if (tokens) DNH_TRY(error_flag_ptr(s, &p.err));
     const PartPlan pp = part_plan(rows, p.vocab, K, (int)sizeof(T));

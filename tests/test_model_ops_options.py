@@ -1,6 +1,8 @@
 """CPU: the switch of the language-model operators, and scratch memory that they do not need."""
 import ctypes as C
 import os
+import re
+import subprocess
 
 import pytest
 
@@ -30,3 +32,10 @@ def test_few_tokens_ask_for_next_to_no_scratch_memory():
     assert n.value > 513 * 8
     native.check(lib.dnh_embedding_grad_scratch_bytes(512, 50000, 1 << 20, C.byref(n)))       # too much for one launch
     assert n.value > 64 * 2 * (1 << 20) * 8
+
+
+def test_attention_kernels_are_those_that_calls_reach():
+    """Two wavefronts take 33 to 64 rows of single precision; in double precision two hold 32, which the kernel for few rows takes."""
+    names = subprocess.run(["nm", native.lib_path()], capture_output=True, text=True, check=True).stdout
+    kernels = re.findall(r"attention_kernelINS_6Mma(F32|F64)ELi(\d+)ELi([24])E", names)
+    assert {(t, w) for t, _, w in kernels} == {("F32", "2"), ("F32", "4"), ("F64", "4")}
