@@ -162,6 +162,7 @@ extern "C" int32_t dnh_cross_attention(const DnhTensor* out, const DnhTensor* ls
     DNH_TRY(check_like(out, q, q->shape[1], q->shape[2], v->shape[3], what, "out", true));
     if (lse) DNH_TRY(check_lse(lse, q, what, true));
     if (nelems(out) == 0) return DNH_OK;
+    DNH_TRY(check_apart<6>({out, lse, q, k, v, mask}, {"out", "lse", "q", "k", "v", "the mask"}, 2, what));
     DNH_TRY(ensure_init());
     return q->dtype == DNH_F32 ? forward<float>(out, lse, q, k, v, mask, scale, scratch, scratch_bytes, (hipStream_t)stream)
                                : forward<double>(out, lse, q, k, v, mask, scale, scratch, scratch_bytes, (hipStream_t)stream);
@@ -183,6 +184,7 @@ extern "C" int32_t dnh_cross_attention_grad(const DnhTensor* d_q, const DnhTenso
         DNH_TRY(check_like(d_v, q, v->shape[1], v->shape[2], v->shape[3], what, "d_v", true));
     }
     if ((!d_q || nelems(d_q) == 0) && (!d_k || nelems(d_k) == 0)) return DNH_OK;
+    DNH_TRY(check_apart<10>({d_q, d_k, d_v, d_out, q, k, v, out, lse, mask}, {"d_q", "d_k", "d_v", "d_out", "q", "k", "v", "out", "lse", "the mask"}, 3, what));
     DNH_TRY(ensure_init());
     return q->dtype == DNH_F32 ? backward<float>(d_q, d_k, d_v, d_out, q, k, v, out, lse, mask, scale, scratch, scratch_bytes, (hipStream_t)stream)
                                : backward<double>(d_q, d_k, d_v, d_out, q, k, v, out, lse, mask, scale, scratch, scratch_bytes, (hipStream_t)stream);

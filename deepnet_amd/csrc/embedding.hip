@@ -738,6 +738,7 @@ extern "C" int32_t dnh_embedding(const DnhTensor* t, const DnhTensor* table, con
     uint32_t n;
     DNH_TRY(check_embedding(table, tokens, t, "dnh_embedding", &n));
     if (n == 0 || table->shape[1] == 0) return DNH_OK;
+    DNH_TRY(check_apart<3>({t, table, tokens}, {"the target", "the table", "tokens"}, 1, "dnh_embedding"));
     DNH_TRY(ensure_init());
     hipStream_t s = (hipStream_t)stream;
     int32_t* err = nullptr;
@@ -768,6 +769,7 @@ extern "C" int32_t dnh_embedding_grad(const DnhTensor* d_table, const DnhTensor*
     if (n > kMaxGradTokens) return fail(DNH_ERR_NOT_SUPPORTED, "dnh_embedding_grad: more than 2^27 tokens");
     if (accumulate != 0 && accumulate != 1) return fail(DNH_ERR_INVALID_ARG, "dnh_embedding_grad: accumulate must be 0 or 1, not %d", accumulate);
     if (d_table->shape[1] == 0 || (d_table->shape[0] == 0 && n == 0)) return DNH_OK;
+    DNH_TRY(check_apart<3>({d_table, tokens, d_out}, {"the gradient of the table", "tokens", "the tensor of rows"}, 1, "dnh_embedding_grad"));
     DNH_TRY(ensure_init());
     return d_table->dtype == DNH_F32 ? embedding_grad<float>(d_table, tokens, d_out, n, scale, accumulate, scratch, scratch_bytes, (hipStream_t)stream)
                                      : embedding_grad<double>(d_table, tokens, d_out, n, scale, accumulate, scratch, scratch_bytes, (hipStream_t)stream);

@@ -656,6 +656,8 @@ extern "C" int32_t dnh_token_log_probs(const DnhTensor* log_probs_t, const DnhTe
     if (rows == 0) return DNH_OK;
     if (logits->shape[nd] == 0) return fail(DNH_ERR_INVALID_ARG, "%s: rows without logits", what);
     if (rows > (1u << 24) - 1) return fail(DNH_ERR_NOT_SUPPORTED, "%s: more than 2^24 - 1 rows", what);
+    DNH_TRY(check_apart<7>({log_probs_t, lse, entropy, top_log_probs, top_tokens, logits, tokens},
+                           {"log_probs", "lse", "entropy", "top_log_probs", "top_tokens", "logits", "tokens"}, 5, what));
     DNH_TRY(ensure_init());
     return logits->dtype == DNH_F32 ? log_probs<float>(log_probs_t, lse, entropy, top_log_probs, top_tokens, logits, tokens, rows, K, scratch, scratch_bytes, (hipStream_t)stream)
                                     : log_probs<double>(log_probs_t, lse, entropy, top_log_probs, top_tokens, logits, tokens, rows, K, scratch, scratch_bytes, (hipStream_t)stream);
@@ -677,6 +679,8 @@ extern "C" int32_t dnh_token_log_probs_grad(const DnhTensor* d_logits, const Dnh
         DNH_TRY(check_per_row(d_entropy, logits, logits->dtype, what, "d_entropy"));
     }
     if (rows == 0 || logits->shape[logits->ndims - 1] == 0) return DNH_OK;
+    DNH_TRY(check_apart<7>({d_logits, same_view(d_logits, logits) ? nullptr : logits, tokens, lse, entropy, d_log_probs, d_entropy},
+                           {"d_logits", "logits", "tokens", "lse", "entropy", "d_log_probs", "d_entropy"}, 1, what));
     DNH_TRY(ensure_init());
     return logits->dtype == DNH_F32 ? log_probs_grad<float>(d_logits, logits, tokens, lse, entropy, d_log_probs, d_entropy, rows, (hipStream_t)stream)
                                     : log_probs_grad<double>(d_logits, logits, tokens, lse, entropy, d_log_probs, d_entropy, rows, (hipStream_t)stream);

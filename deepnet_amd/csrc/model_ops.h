@@ -78,6 +78,85 @@ inline int32_t check_target(const DnhTensor* t, const char* what, const char* na
     return DNH_OK;
 }
 
+// ---- targets that share memory with a source or with each other ------------------------------------------------------------------
+// Whether two views certainly have a byte in common: both fill the ranges they span, and those meet; or a corner of one (its first or last
+// position along every axis) is an element of the other.  Views that interleave (heads beside each other in one tensor) do not count.
+struct Span {
+    int64_t lo = 0, hi = 0;   // addresses of the first and behind the last byte
+    int nd = 0;               // axes of more than one position, by descending stride, all positive
+    int64_t n[DNH_MAX_DIMS], stride[DNH_MAX_DIMS];
+    bool nested = true;       // every stride is longer than what the axes behind it reach: positions and addresses are one to one
+    int esize = 0;
+};
+inline Span span_of(const DnhTensor* t) {
+    Span s;
+    s.esize = dtype_size(t->dtype);
+    s.lo = (int64_t)(intptr_t)t->base + t->offset * s.esize;
+    int64_t last = 0;
+    for (int d = 0; d < t->ndims; d++) {
+        if (t->shape[d] < 2 || t->stride[d] == 0) continue;
+        const int64_t st = (t->stride[d] < 0 ? -t->stride[d] : t->stride[d]) * s.esize, reach = st * (t->shape[d] - 1);
+        if (t->stride[d] < 0) s.lo -= reach;
+        last += reach;
+        int at = s.nd++;
+        for (; at > 0 && s.stride[at - 1] < st; at--) {
+            s.stride[at] = s.stride[at - 1];
+            s.n[at] = s.n[at - 1];
+        }
+        s.stride[at] = st;
+        s.n[at] = t->shape[d];
+    }
+    s.hi = s.lo + last + s.esize;
+    int64_t inner = s.esize;
+    for (int d = s.nd - 1; d >= 0; d--) {
+        if (s.stride[d] < inner) s.nested = false;
+        inner += s.stride[d] * (s.n[d] - 1);
+    }
+    return s;
+}
+inline bool fills(const Span& s) {
+    int64_t bytes = s.esize;
+    for (int d = 0; d < s.nd; d++) bytes *= s.n[d];
+    return s.nested && bytes == s.hi - s.lo;
+}
+inline bool has_corner_of(const Span& a, const Span& b) {   // equal element sizes
+    if (!a.nested) return false;
+    for (int c = 0; c < 1 << b.nd; c++) {
+        int64_t at = b.lo - a.lo;
+        for (int d = 0; d < b.nd; d++)
+            if ((c >> d) & 1) at += b.stride[d] * (b.n[d] - 1);
+        bool in = at >= 0;
+        for (int d = 0; d < a.nd && in; d++) {
+            const int64_t i = at / a.stride[d];
+            in = i < a.n[d];
+            at -= i * a.stride[d];
+        }
+        if (in && at == 0) return true;
+    }
+    return false;
+}
+inline bool surely_overlap(const Span& a, const Span& b) {
+    if (a.hi <= b.lo || b.hi <= a.lo) return false;
+    if (fills(a) && fills(b)) return true;
+    return a.esize == b.esize && (has_corner_of(a, b) || has_corner_of(b, a));
+}
+inline bool same_view(const DnhTensor* x, const DnhTensor* y) {
+    if (x->base != y->base || x->offset != y->offset || x->ndims != y->ndims || x->dtype != y->dtype) return false;
+    for (int d = 0; d < x->ndims; d++)
+        if (x->shape[d] != y->shape[d] || (x->shape[d] > 1 && x->stride[d] != y->stride[d])) return false;
+    return true;
+}
+// targets before sources; any may be NULL
+template <int N> int32_t check_apart(const DnhTensor* const (&ts)[N], const char* const (&names)[N], int targets, const char* what) {
+    Span s[N];
+    for (int i = 0; i < N; i++)
+        if (ts[i] && nelems(ts[i]) > 0) s[i] = span_of(ts[i]);   // (else an empty range, which meets none)
+    for (int i = 0; i < targets; i++)
+        for (int j = i + 1; j < N; j++)
+            if (surely_overlap(s[i], s[j])) return fail(DNH_ERR_INVALID_ARG, "%s: %s overlaps %s in memory", what, names[i], names[j]);
+    return DNH_OK;
+}
+
 inline int32_t check_float(const DnhTensor* t, int32_t dtype, const char* what, const char* name) {
     if (!dtype_is_fp(t->dtype)) return fail(DNH_ERR_NOT_SUPPORTED, "%s on %s", what, dtype_name(t->dtype));
     if (t->dtype != dtype) return fail(DNH_ERR_INVALID_ARG, "%s: %s is %s, not %s", what, name, dtype_name(t->dtype), dtype_name(dtype));

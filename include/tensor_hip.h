@@ -336,7 +336,8 @@ int32_t dnh_symmetric_eig(int32_t part, const DnhTensor* eigvals, const DnhTenso
  * Operators of language models (no counterpart in ITensorBackend): token embedding, token log probabilities, cross attention, each
  * with its gradient.  Single and double precision, int64 tokens, any strides and offsets.
  *  - `scale` points to one host element of the operands' type, as `value` of dnh_fill_const does; NULL selects the default;
- *  - targets may not be broadcast views and, unless a declaration says so, may not overlap a source;
+ *  - targets may not be broadcast views and, unless a declaration says so, may not overlap a source or each other.  Where both fill the ranges of
+ *    memory they span, or a corner of one is an element of the other, the call is refused; views that cross in other ways are the caller's care;
  *  - `scratch` is device memory for the call's intermediates, aligned to 16 bytes, of at least the number of bytes that the
  *    operator's dnh_*_scratch_bytes reports; it must stay untouched until the call's kernels have run.  NULL: the library uses the
  *    stream's workspace.  While the stream is being captured into a graph, a call that needs scratch memory is refused without it
