@@ -399,7 +399,7 @@ __device__ __forceinline__ void cut2(float x, float y, uint32_t& hi, uint32_t& m
     y -= __uint_as_float(mid & 0xFFFF0000u);
     lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{x, y}), B2));
 }
-template <int DP, int WAVES, bool PIN> struct AttOpsX3 {
+template <int DP, int WAVES> struct AttOpsX3 {
     using Mma = MmaF32;
     using T = float;
     using Acc = MmaF32::Acc;
@@ -484,14 +484,10 @@ template <int DP, int WAVES, bool PIN> struct AttOpsX3 {
             put3(b.x, st.b[j]);
         }
     }
-    // PIN: reads stay ahead of the matrix instructions (as above), which go before the other wavefront's softmax.  Not so in the gradient up to
-    // width 64, which has no registers to read ahead into: 594 us pinned, 560 us as the compiler orders it (16 x 16 heads, 512 queries, 1024 keys).
-    static __device__ __forceinline__ void pin() {
-        if constexpr (PIN) __builtin_amdgcn_sched_barrier(0x6);
-    }
-    template <int P> static __device__ __forceinline__ void hold() {
-        if constexpr (PIN) __builtin_amdgcn_s_setprio(P);
-    }
+    // Reads stay ahead of the matrix instructions (as above), which go before the other wavefront's softmax: gradient of 16 x 16 heads, 512 queries,
+    // 1024 keys at width 64 580 us, 595 us as the compiler orders it; at width 32 (8 x 16 heads) 152 and 155 us.
+    static __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0x6); }
+    template <int P> static __device__ __forceinline__ void hold() { __builtin_amdgcn_s_setprio(P); }
     static __device__ __forceinline__ Acc mfma(const Bf8& a, const Bf8& b, const Acc& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     // c += a . b, the smallest products first
     static __device__ __forceinline__ void six(Acc& c, const Bf8 (&a)[3], const Bf8& b0, const Bf8& b1, const Bf8& b2) {
@@ -603,11 +599,11 @@ template <int DP, int WAVES, bool PIN> struct AttOpsX3 {
     }
 };
 // What a kernel runs first, and what instead if that fails: the same type where it cannot.
-template <class A, int DP, int WAVES, bool WHOLE, bool PIN> struct AttFirst {
+template <class A, int DP, int WAVES, bool WHOLE> struct AttFirst {
     typedef AttOps<A, DP, WAVES, WHOLE> Ops;
 };
-template <int DP, int WAVES, bool PIN> struct AttFirst<MmaF32, DP, WAVES, true, PIN> {
-    typedef AttOpsX3<DP, WAVES, PIN> Ops;
+template <int DP, int WAVES> struct AttFirst<MmaF32, DP, WAVES, true> {
+    typedef AttOpsX3<DP, WAVES> Ops;
 };
 
 // ---- the softmax of one tile ----------------------------------------------------------------------------------------------------------
@@ -772,7 +768,7 @@ __device__ __forceinline__ bool att_forward(const AttArgs<typename Ops::T>& p, A
 }
 template <class A, int DP, int WAVES, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel(AttArgs<typename A::T> p) {
-    using First = typename AttFirst<A, DP, WAVES, WHOLE, true>::Ops;
+    using First = typename AttFirst<A, DP, WAVES, WHOLE>::Ops;
     using Exact = AttOps<A, DP, WAVES, WHOLE>;
     __shared__ union {
         AttLds<First> first;
@@ -1172,7 +1168,7 @@ __device__ __forceinline__ bool att_dkv(const AttArgs<typename Ops::T>& p, GradL
 // at width 64 in 563 us (999 us).  At width 96 and 128 one wavefront a SIMD has no other to hide its vector instructions behind.
 template <class A, int DP, bool WHOLE>
 __global__ __launch_bounds__(64 * kGradWaves, DP <= 64 ? 2 : 1) void attention_grad_kernel(AttArgs<typename A::T> p, uint32_t first, bool dq_first) {
-    using First = typename AttFirst<A, DP, kGradWaves, WHOLE, (DP > 64)>::Ops;
+    using First = typename AttFirst<A, DP, kGradWaves, WHOLE>::Ops;
     using Exact = AttOps<A, DP, kGradWaves, WHOLE>;
     __shared__ union {
         GradLds<First> first;
