@@ -406,7 +406,7 @@ template <int DP, int WAVES> struct AttOpsX3 {
     using V = Vec16<float>::type;
     static constexpr int M = 32, NS = 1, ND = DP / 32, NT = DP / 16;
     // LDS rows of 20 or 52 words beyond a multiple of 64: 16 rows' 16-byte reads fall on different banks, and the four rows of a transposed read
-    // overlap little (width 128, 4 words: 355 us of gradient instead of 347).  At width 64 two workgroups have no room for that: 36 words.
+    // overlap little (width 128, 4 words: 311 us forward instead of 304, 330 us of gradient instead of 328).  At width 64 two workgroups have no room for that: 36 words.
     static constexpr int P = DP == 128 ? 168 : DP + 8, PLANE = kAttTile * P;
     typedef uint32_t U2 __attribute__((ext_vector_type(2)));
     typedef uint32_t U4 __attribute__((ext_vector_type(4)));
@@ -691,8 +691,9 @@ __device__ __forceinline__ void att_store(const AttArgs<typename Ops::T>& p, con
 // that writes buffer b has passed the barrier behind everybody's last reads of it).
 // Bound by the matrix pipes and the vector instructions that the wavefronts of a SIMD do not hide behind them (softmax, cutting P and the
 // staged tiles): 8 x 16 heads, 512 queries, up to 1500 keys at width 64 take 126 us, pipes busy half the time (196 us on the float
-// instructions, pipes busy 72 %).  Two wavefronts a workgroup only where four would not have rows: 712 us instead of 650 for 2000 queries
-// when the float instructions did it all.
+// instructions, pipes busy 72 %).  Two wavefronts a workgroup only where four would not have rows, in single precision from 33 to 64: 40 queries
+// over 60 000 keys of 2 heads 35.5 us, four wavefronts 37.4, but 33 queries over 2000 keys of 64 heads 34.0 and 31.1.  Beyond, four: 2000 queries
+// of 32 heads 143 us, two wavefronts 242.
 template <class Ops> struct AttLds {
     typename Ops::Tile k[2], v[2];
     uint32_t words[kAttWords];
@@ -784,7 +785,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 2 : 1) void attention_kernel
 // Bound by the bytes of the keys and values: 32 keys at width 64 are 2048 cycles of the matrix pipe and 16 KB, i.e. the pipes keep up with
 // three times the memory's rate.  A lane of value row `key` loads elements 16-byte-wise and uses element e of load g for
 // accumulator E g + e: accumulator i holds the elements E 16 g + E row + e of the result.
-// 16 sequences of up to 2000 keys, 4 key heads at width 64 (47 MB): 12.7 to 14.7 us, and 4.4 us for joining the shares.  The float instructions
+// 16 sequences of up to 2000 keys, 4 key heads at width 64 (47 MB): 14 to 15 us, and 4 us for joining the shares.  The float instructions
 // stay here: cutting a tile that one wavefront uses once costs more than it saves.
 template <class A, int DP, bool WHOLE>
 __global__ __launch_bounds__(64) void attention_few_kernel(AttArgs<typename A::T> p) {
@@ -888,7 +889,7 @@ __global__ __launch_bounds__(64) void attention_few_kernel(AttArgs<typename A::T
 
 // Joins the shares of each row, first their weights across the lanes, then lanes along the width: a wavefront per row or, with many shares, the
 // four of a workgroup, whose sums are added in order.  A launch and two dependent reads: 4.4 us for 256 rows of 32 shares (a wavefront each 5.5).
-// One query of a long sequence needs many shares: 100 000 keys of 2 heads at width 64 take 38 us with 256 shares, 101 us with 64.
+// One query of a long sequence needs many shares: 100 000 keys of 2 heads at width 64 take 37 us with 256 shares, 101 us with 64.
 constexpr uint32_t kMaxShares = 256;
 template <class A, bool WIDE>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs<typename A::T> p) {
@@ -1164,8 +1165,8 @@ __device__ __forceinline__ bool att_dkv(const AttArgs<typename Ops::T>& p, GradL
 // Both halves of the backward pass in one launch, so that neither leaves compute units idle while the other runs out: `first` workgroups of
 // dq (dq_first) or of dk and dv, then those of the other.  The half with the longer walks goes first: what is left for the end is short.
 // Bound as the forward pass, with seven products of a tile instead of two (S and dP are computed in both halves: dS kept by
-// one for the other would be memory of rows x keys): 4 x 16 heads, 512 queries, 1024 keys at width 128 in 345 us (float instructions: 521 us), 16 x 16 heads
-// at width 64 in 563 us (999 us).  At width 96 and 128 one wavefront a SIMD has no other to hide its vector instructions behind.
+// one for the other would be memory of rows x keys): 4 x 16 heads, 512 queries, 1024 keys at width 128 in 323 us with the launch for delta (float instructions: 493 us), 16 x 16 heads
+// at width 64 in 550 to 580 us (910 to 930 us).  At width 96 and 128 one wavefront a SIMD has no other to hide its vector instructions behind.
 template <class A, int DP, bool WHOLE>
 __global__ __launch_bounds__(64 * kGradWaves, DP <= 64 ? 2 : 1) void attention_grad_kernel(AttArgs<typename A::T> p, uint32_t first, bool dq_first) {
     using First = typename AttFirst<A, DP, kGradWaves, WHOLE>::Ops;
@@ -1213,7 +1214,11 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(AttArgs<T> p, 
 
 // ---- plan and launch ------------------------------------------------------------------------------------------------------------------------
 constexpr uint32_t kAttCUs = 256;   // MI355X; a constant, so that the size of the scratch memory can be asked for without a device
-constexpr int64_t kFewRows = 32;    // up to here the kernel without LDS (two blocks of 16 rows read the keys twice, the second time from the L2)
+// Up to here the kernel without LDS (two blocks of 16 rows read the keys twice, the second time from the L2).  It against the tiles, in us: 2000 keys of
+// 64 heads at width 64, 16 rows 20 and 34, 32 rows 25 and 34, 33 rows 35 and 34, 64 rows 36 and 36, 96 rows 57 and 35; 1500 keys of 256 heads 32 rows 50
+// and 73, 64 rows 112 and 78; 200 keys of 128 heads 32 rows 15 and 17, 64 rows 20 and 20; at width 128 (2000 keys of 64 heads) 32 rows 47 and 83, 64
+// rows 73 and 85.  Double precision, 16 rows 34 and 45, 32 rows 47 and 47, 33 rows 58 and 56 (64 heads).
+constexpr int64_t kFewRows = 32;
 
 // Shares of a walk over `tiles` tiles, at least two tiles each and at most `most` shares, until `want` workgroups are reached.
 inline void att_shares(int64_t workgroups, int64_t tiles, int64_t want, int64_t most, uint32_t* shares, uint32_t* share_tiles) {
@@ -1231,8 +1236,9 @@ inline void att_shares(int64_t workgroups, int64_t tiles, int64_t want, int64_t 
 // Estimates in microseconds that choose the numbers of shares, fitted to 512 queries and 1024 keys at widths 32 to 128: a 32-row tile costs a
 // wavefront 0.0105 us a product and column in single precision and 0.0145 in double precision (matrix instructions, and what cutting, staging and
 // softmax leave uncovered), and 0.3 or 1 us besides; starting and ending a workgroup 4 us.  Up to padded width 64 two workgroups of
-// four wavefronts fit a compute unit (they share the pipes), above one.  Shares chosen so, against a fixed target of 256 workgroups, when the
-// float instructions did the products: 300 queries over 3000 keys at width 128 258 -> 174 us.
+// four wavefronts fit a compute unit (they share the pipes), above one.  With shares chosen so, with as many as make 256 workgroups, and with none, in us: 300
+// queries over 3000 keys of 4 heads at width 128 35, 35 and 290, their gradient 81, 111 and 322; 40 queries over 60 000 keys of 2 heads 35, 48 and 3827;
+// 33 over 2000 of 64 heads 34, 48 and 150; 513 over 2000 of 16 heads 46, 54 and 110; 1000 x 1000 of 8 heads 31, 31 and 58, their gradient 64, 62 and 128.
 inline int att_resident(int64_t width) { return width <= 64 ? 2 : 1; }
 template <class T> double att_walk_us(int64_t width, int products, int64_t tiles) {
     const double padded = (double)((width + 31) / 32 * 32), column = sizeof(T) == 4 ? 0.0105 : 0.0145, tile = sizeof(T) == 4 ? 0.3 : 1.0;

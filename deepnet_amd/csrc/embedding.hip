@@ -1,7 +1,7 @@
 // dnh_embedding, dnh_embedding_grad: rows of a table by token number, scaled, and the gradient of the table.
 //
 //   t[i, :]       = scale * table[tokens[i], :]
-//   d_table[v, :] = scale * sum over { i : tokens[i] = v } of d_out[i, :]      (the sum in 64 bits, in the order of i; one rounding)
+//   d_table[v, :] = scale * sum over { i : tokens[i] = v } of d_out[i, :]      (the sum in 64 bits, in an order that depends on the tokens alone; one rounding)
 //
 // Both are bound by HBM: the lookup reads every row it names and writes N x D, the gradient reads N x D and writes V x D.
 // The gradient needs no atomics: the N token numbers are sorted (stable, with their positions) and each run of equal tokens is added up
@@ -479,8 +479,8 @@ __global__ __launch_bounds__(kJoinThreads) void embedding_join_kernel(GradTarget
 // Up to kFewTokens everything in one launch, without a sort: each workgroup reads all the tokens.  Those of leader i add up the rows of the
 // tokens equal to the i-th unless one before it is equal, 16 bytes of the row per lane, equal tokens dealt to four wavefronts whose sums
 // are added in order.  The others clear blocks of rows, leaving out those that a leader writes.  Bound by latency: the tokens, the rows, the sums.
-// 512 tokens into 10 007 rows of 300 floats 8.6 us against 15.7 us sorted (513 tokens), 16 tokens 7.6 us; into 50 000 rows of 1024 (205 MB to
-// clear) 40 us against 47; 500 tokens into 500 rows of 2000, where the sums are most of it, 12.4 us against 14.3.
+// 512 tokens into 10 007 rows of 300 floats 8.4 us against 16.3 us sorted (513 tokens), 16 tokens 7.5 us; into 50 000 rows of 1024 (205 MB to
+// clear) 45 us against 48.5; into 500 rows of 2000, where the sums are most of it, 12.4 us against 15.6 (in double precision 16.1 against 15.6).
 constexpr uint32_t kFewTokens = 512;
 constexpr int kFillRows = 2048;   // most rows of a block that is cleared at once
 constexpr size_t kFewScratch = 256;   // what the query answers for them: none of it is used, but a call with less than the query says is refused

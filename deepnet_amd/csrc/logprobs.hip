@@ -19,7 +19,7 @@ namespace {
 constexpr int kBlock = 256, kWaves = kBlock / 64;
 constexpr int kMaxTop = 64;                     // one alternative per lane of a wavefront
 constexpr uint32_t kNoIndex = 0xFFFFFFFFu;
-constexpr int kSlice = 4096;                    // fewest elements of a row that a workgroup takes when a row is shared
+constexpr int kSlice = 4096;                    // a row is shared among no more workgroups than have this many elements, but for the last one's rest
 
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896340736f); }
 __device__ __forceinline__ double exp_of(double d) { return exp(d); }
@@ -287,7 +287,7 @@ __device__ __forceinline__ double shrink(double d, float) {
 __device__ __forceinline__ double shrink(double d, double) { return exp(d); }
 
 // A workgroup takes elements [j0, j1) of a row.  With one workgroup per row it writes the results, else its statistics and list.
-// Without alternatives it runs at the memory's rate: 4096 rows of 50 048 floats (820 MB) in 127 us, 6.5 TB/s.  With 5 alternatives 149 us: sorting
+// Without alternatives it runs at the memory's rate: 4096 rows of 50 048 floats (820 MB) in 127 us, 6.5 TB/s.  With 5 alternatives 149 to 152 us: sorting
 // the start of a row and inserting what passes the floor later take turns with the loads of the same wavefront.  One row of 128 000 with 20
 // alternatives is a chain of latencies: 32 slices in 11 us, joined in 9 us.
 template <class T, bool VEC, bool TOP>
@@ -427,7 +427,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void log_probs_join_kernel(LogProb
 }
 
 // Workgroups that share a row.  A workgroup per row fills the chip from about two rows per compute unit on; below that the rows are cut
-// into slices of at least kSlice elements, until there are about four workgroups per compute unit.
+// into slices, one for each kSlice elements at most and all of about one length, until there are about four workgroups per compute unit.
 constexpr uint32_t kCUs = 256;   // MI355X; a constant, so that the size of the scratch memory can be asked for without a device
 uint32_t split_count(uint32_t rows, int64_t vocab) {
     const int64_t want = (4 * kCUs + rows - 1) / rows, most = (vocab + kSlice - 1) / kSlice;
