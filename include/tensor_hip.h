@@ -383,7 +383,7 @@ int32_t dnh_token_log_probs_grad(const DnhTensor* d_logits, const DnhTensor* log
  * Widths up to 128.  [B; L; H; D] tensors are passed as permuted views.  Single precision: where widths are multiples of 4 along contiguous
  * axes the products are taken on the bf16 matrix instructions from three parts of every number, with the error of a float product; a
  * workgroup that meets an element below 2^-109 (zero apart), or whose sums are not finite, takes the float instructions, as all do with the option
- * "attention_bf16x3" = 0.  Before they are divided by
+ * "attention_bf16x3" = 0.  Probabilities below 2^-126 count as zero, and three parts hold the others to 2^-134.  Before they are divided by
  * their denominator, sums over the keys of e^(score - largest score) |v| must stay in the type's range. */
 int32_t dnh_cross_attention(const DnhTensor* out, const DnhTensor* lse, const DnhTensor* q, const DnhTensor* k, const DnhTensor* v,
                             const DnhTensor* mask_bool, const void* scale, void* scratch, size_t scratch_bytes, void* stream);
